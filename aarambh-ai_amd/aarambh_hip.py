@@ -29,6 +29,10 @@ LIB_PATH = os.path.join(_HERE, "libaarambh_hip.so")
 
 W_F32, W_BF16, W_INT8_ROW, W_INT4_G128 = 0, 1, 2, 3
 KV_F32, KV_F16, KV_INT8 = 0, 1, 2
+KV_BF16 = 3  # page pools only
+A_F32, A_F16, A_BF16 = 0, 1, 2
+DEFAULT_STREAM = 1
+SEQ_BAD_PAGE, SEQ_BAD_LENGTH = 1, 2
 T_NORM, T_LINEAR, T_EMBED = 0, 1, 2
 FLAG_RATIO_NEAR, FLAG_CDF_NEAR, FLAG_TOPP_NEAR = 1, 2, 8
 TOP_CANDIDATES = 5  # engine.rs:70
@@ -99,8 +103,41 @@ class _Stats(C.Structure):
                                           "draft_decode_forwards", "mtp_head_forwards")]
 
 
-_lib = None
 _P = C.c_void_p
+
+
+class _PagePool(C.Structure):
+    _fields_ = [(n, C.c_int32) for n in ("kv_format", "n_kv_heads", "head_dim", "page_tokens", "n_pages")] + \
+               [(n, _P) for n in ("k", "v", "k_scale", "v_scale")]
+
+
+class _PageBatch(C.Structure):
+    _fields_ = [(n, C.c_int32) for n in ("nseq", "rows", "max_rows", "max_kv")] + \
+               [(n, _P) for n in ("row_off", "kv_len", "tables")] + [("table_ld", C.c_int64), ("status", _P)]
+
+
+class _RopeArgs(C.Structure):
+    _fields_ = [("act", C.c_int32), ("n_heads", C.c_int32), ("q", _P), ("k", _P), ("v", _P), ("q_ld", C.c_int64),
+                ("k_ld", C.c_int64), ("v_ld", C.c_int64), ("q_out", _P), ("q_out_ld", C.c_int64), ("inv_freq", _P),
+                ("rot_dim", C.c_int32), ("interleaved", C.c_int32), ("attn_factor", C.c_float)]
+
+
+class _PagedAttnArgs(C.Structure):
+    _fields_ = [("act", C.c_int32), ("n_heads", C.c_int32), ("grouped", C.c_int32), ("q", _P), ("q_ld", C.c_int64),
+                ("out", _P), ("out_ld", C.c_int64), ("scale", C.c_float), ("softcap", C.c_float),
+                ("window", C.c_int32), ("slopes", _P), ("prefix", _P), ("workspace", _P),
+                ("workspace_bytes", C.c_int64)]
+
+
+class _LogitsArgs(C.Structure):
+    _fields_ = [("nseq", C.c_int32), ("rows_per_seq", C.c_int32), ("vocab", C.c_int32), ("logits", _P),
+                ("ld", C.c_int64), ("out", _P), ("out_ld", C.c_int64), ("history", _P), ("history_ld", C.c_int64),
+                ("history_len", _P), ("prompt_len", _P), ("penalties", _P), ("draft", _P), ("draft_ld", C.c_int64),
+                ("bias_off", _P), ("bias_ids", _P), ("bias_vals", _P), ("n_bias", C.c_int32), ("masks", _P),
+                ("mask_ld", C.c_int64), ("n_masks", C.c_int32), ("mask_of_row", _P)]
+
+
+_lib = None
 
 
 def lib():
@@ -200,6 +237,14 @@ def lib():
         "aarh_lat_forward": (C.c_int, [_P, _P, _P, _P, C.c_int, C.c_int, _P, _P]),
         "aarh_lat_router_gaps": (C.c_int, [_P, _P]),
         "aarh_lat_expert_counts": (C.c_int, [_P, _P]),
+        "aarh_rope_append": (C.c_int, [_P, C.POINTER(_PagePool), C.POINTER(_PageBatch), C.POINTER(_RopeArgs), _P]),
+        "aarh_rope_frequencies": (C.c_int, [C.c_int32, C.c_double, C.c_int32, C.POINTER(_RopeScaling), _P,
+                                            C.POINTER(C.c_float)]),
+        "aarh_paged_attention": (C.c_int, [_P, C.POINTER(_PagePool), C.POINTER(_PageBatch),
+                                           C.POINTER(_PagedAttnArgs), _P]),
+        "aarh_paged_attention_workspace": (C.c_int, [_P, C.POINTER(_PagePool), C.POINTER(_PageBatch),
+                                                     C.POINTER(_PagedAttnArgs), C.POINTER(C.c_int64)]),
+        "aarh_process_logits": (C.c_int, [_P, C.POINTER(_LogitsArgs), _P]),
         "aarh_lat_prof_enable": (C.c_int, [_P, C.c_int]),
         "aarh_lat_prof_get": (C.c_int, [_P, C.c_int, C.POINTER(C.c_double), C.POINTER(C.c_double),
                                         C.POINTER(C.c_int64)]),
@@ -231,7 +276,8 @@ EXPORTED = ["aarh_create", "aarh_destroy", "aarh_last_error", "aarh_stream", "aa
             "aarh_spec_session_step", "aarh_spec_session_result", "aarh_spec_session_candidates",
             "aarh_spec_session_rng_offsets", "aarh_spec_session_set_rng_offsets", "aarh_spec_session_end",
             "aarh_set_rope_scaling", "aarh_gguf_rope_scaling", "aarh_lat_get_config", "aarh_lat_load_gguf",
-            "aarh_lat_load_safetensors", "aarh_lat_gguf_config"]
+            "aarh_lat_load_safetensors", "aarh_lat_gguf_config", "aarh_rope_append", "aarh_rope_frequencies",
+            "aarh_paged_attention", "aarh_paged_attention_workspace", "aarh_process_logits"]
 
 
 def _ptr(a):
@@ -321,6 +367,122 @@ class RopeScaling:
             raise ConfigError(f"unknown rope_scaling method {self.method!r}")
         return _RopeScaling(ROPE_METHODS[self.method], int(self.original_max_seq_len), float(self.factor),
                             float(self.beta_fast), float(self.beta_slow), float(self.attn_factor))
+
+
+def rope_frequencies(rot_dim, theta=10000.0, scaling: Optional[RopeScaling] = None, max_seq_len=0):
+    """Inverse frequencies [rot_dim / 2] in f64 and the cos / sin factor under `scaling`, for
+    HipModel.rope_append (aarh_rope_frequencies)."""
+    inv = np.zeros(max(int(rot_dim) // 2, 1), np.float64)
+    attn = C.c_float()
+    s = scaling._c() if scaling is not None else None
+    _host_check(lib().aarh_rope_frequencies(int(rot_dim), float(theta), int(max_seq_len),
+                                            None if s is None else C.byref(s), _ptr(inv), C.byref(attn)))
+    return inv, attn.value
+
+
+def _on(device, name, t, dtype, dim, contiguous=True):
+    """Data pointer of a device tensor (None: NULL) after its checks."""
+    if t is None:
+        return None
+    if t.device.type != "cuda" or t.device.index != device:
+        raise ConfigError(f"{name} must be on cuda:{device}, not {t.device}")
+    if t.dtype != dtype:
+        raise UnsupportedError(f"{name} must be {dtype}, not {t.dtype}")
+    if t.dim() != dim:
+        raise ShapeError(f"{name} must have {dim} dimensions, not {t.dim()}")
+    if contiguous and not t.is_contiguous():
+        raise UnsupportedError(f"{name} must be contiguous")
+    return t.data_ptr()
+
+
+def _stream(device):
+    """The current torch stream as the C ABI takes it (the default stream has a value of its own there)."""
+    import torch
+    return torch.cuda.current_stream(device).cuda_stream or DEFAULT_STREAM
+
+
+class PagePool:
+    """Pages of a key / value cache (aarh_page_pool): k, v [n_pages, n_kv_heads, page_tokens * head_dim] of
+    torch.float16, bfloat16 or int8 on one device, INT8 with k_scale, v_scale [n_pages, n_kv_heads, page_tokens]
+    float16.  The order of the elements within a page is the operators' own; read() gives tokens back."""
+
+    def __init__(self, k, v, n_kv_heads, head_dim, page_tokens, k_scale=None, v_scale=None):
+        import torch
+        fmt = {torch.float16: KV_F16, torch.bfloat16: KV_BF16, torch.int8: KV_INT8}.get(k.dtype)
+        if fmt is None:
+            raise UnsupportedError(f"page pools hold float16, bfloat16 or int8, not {k.dtype}")
+        dev = k.device.index
+        want = (k.shape[0], n_kv_heads, page_tokens * head_dim)
+        for name, t in (("k", k), ("v", v)):
+            _on(dev, name, t, k.dtype, 3)
+            if tuple(t.shape) != want:
+                raise ShapeError(f"{name} must be {want}, not {tuple(t.shape)}")
+        if (fmt == KV_INT8) != (k_scale is not None) or (fmt == KV_INT8) != (v_scale is not None):
+            raise ConfigError("INT8 pools, and only these, have k_scale and v_scale")
+        for name, t in (("k_scale", k_scale), ("v_scale", v_scale)):
+            _on(dev, name, t, torch.float16, 3)
+            if t is not None and tuple(t.shape) != (k.shape[0], n_kv_heads, page_tokens):
+                raise ShapeError(f"{name} must be {(k.shape[0], n_kv_heads, page_tokens)}, not {tuple(t.shape)}")
+        self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
+        self.kv_format, self.n_kv_heads, self.head_dim, self.page_tokens = fmt, n_kv_heads, head_dim, page_tokens
+        self.device = dev
+        p = lambda t: None if t is None else t.data_ptr()  # noqa: E731
+        self._c = _PagePool(fmt, n_kv_heads, head_dim, page_tokens, k.shape[0], p(k), p(v), p(k_scale), p(v_scale))
+
+    @classmethod
+    def allocate(cls, n_pages, n_kv_heads, head_dim, page_tokens=64, kv_format=KV_F16, device=0):
+        import torch
+        dt = {KV_F16: torch.float16, KV_BF16: torch.bfloat16, KV_INT8: torch.int8}.get(kv_format)
+        if dt is None:
+            raise UnsupportedError(f"page pools hold KV_F16, KV_BF16 or KV_INT8, not format {kv_format}")
+        new = lambda *shape, dtype: torch.zeros(shape, dtype=dtype, device=f"cuda:{device}")  # noqa: E731
+        kv = [new(n_pages, n_kv_heads, page_tokens * head_dim, dtype=dt) for _ in range(2)]
+        sc = [new(n_pages, n_kv_heads, page_tokens, dtype=torch.float16) if kv_format == KV_INT8 else None
+              for _ in range(2)]
+        return cls(*kv, n_kv_heads, head_dim, page_tokens, *sc)
+
+    def read(self, pages):
+        """Keys and values of a list of pages, [n * page_tokens, n_kv_heads, head_dim] f32."""
+        import torch
+        at = torch.as_tensor(pages, dtype=torch.long, device=self.k.device)
+        n, nb, hd, nkv = at.numel(), self.page_tokens // 32, self.head_dim, self.n_kv_heads
+        if self.kv_format == KV_INT8:  # [s][c][g][a][b][h][j] and [p][g][r][h][j]
+            k = self.k[at].reshape(n, nkv, nb, 2, hd // 64, 4, 4, 4, 2, 8).permute(0, 2, 6, 3, 7, 1, 4, 5, 8, 9)
+            v = self.v[at].reshape(n, nkv, nb, hd // 32, 4, 16, 2, 8).permute(0, 2, 4, 7, 1, 3, 6, 5)
+        else:  # [s][c][h][g][a][b][j] and [d][t]
+            k = self.k[at].reshape(n, nkv, nb, 2, hd // 64, 2, 4, 4, 4, 8).permute(0, 2, 7, 3, 8, 1, 4, 6, 5, 9)
+            v = self.v[at].reshape(n, nkv, nb, hd, 32).permute(0, 2, 4, 1, 3)
+        out = []
+        for x, sc in ((k, self.k_scale), (v, self.v_scale)):
+            x = x.reshape(n * self.page_tokens, nkv, hd).float()
+            if sc is not None:
+                x = x * sc[at].permute(0, 2, 1).reshape(-1, nkv, 1).float()
+            out.append(x)
+        return out
+
+
+class PageBatch:
+    """The sequences of one call (aarh_page_batch): tables [nseq, table_ld] int32 page numbers, kv_len [nseq]
+    int32, row_off [nseq + 1] int32, all on the device; `rows` of the activation buffers, bounds max_rows
+    and max_kv; status [nseq] int32 (optional) takes SEQ_* bits."""
+
+    def __init__(self, tables, kv_len, row_off, rows, max_rows, max_kv, status=None):
+        import torch
+        dev = tables.device.index
+        n = kv_len.shape[0]
+        for name, t, dim in (("tables", tables, 2), ("kv_len", kv_len, 1), ("row_off", row_off, 1), ("status", status, 1)):
+            _on(dev, name, t, torch.int32, dim, contiguous=name != "tables")
+        if tables.shape[0] != n or row_off.shape[0] != n + 1 or (status is not None and status.shape[0] != n):
+            raise ShapeError(f"{n} sequences, but {tables.shape[0]} tables and {row_off.shape[0]} row offsets")
+        if tables.shape[1] > 1 and tables.stride(1) != 1:
+            raise UnsupportedError("a page table's entries must be contiguous")
+        self.tables, self.kv_len, self.row_off, self.status, self.device = tables, kv_len, row_off, status, dev
+        self.rows = rows
+        self.entries = tables.shape[1]
+        p = lambda t: None if t is None else t.data_ptr()  # noqa: E731
+        self._c = _PageBatch(n, rows, max_rows, max_kv, p(row_off), p(kv_len), p(tables),
+                             tables.stride(0) if n > 1 else tables.shape[1], p(status))
+        self._workspace = {}
 
 
 @dataclass
@@ -459,6 +621,7 @@ class HipModel:
                  cfg.max_seq_len, cfg.rope_theta, cfg.norm_eps, cfg.num_future_tokens, cfg.weight_format,
                  cfg.lm_head_format, cfg.kv_format, max_batch, max_rows, 0 if cfg.tie_embeddings else 1)
         h = _P()
+        self.device = device
         st = lib().aarh_create(device, C.byref(c), C.byref(h))
         self.h = h
         if st:
@@ -637,6 +800,144 @@ class HipModel:
         self._check(st)
         self.sync()
         return outs
+
+
+    # ------------------------------------------------------------------
+    # operators over paged caches and on logits: device tensors, the current torch stream
+    # ------------------------------------------------------------------
+    def _act(self, name, t, rows, heads, hd):
+        """(activation format, row stride) of a [rows, heads, head_dim] tensor whose rows may be apart."""
+        import torch
+        act = {torch.float32: A_F32, torch.float16: A_F16, torch.bfloat16: A_BF16}.get(t.dtype)
+        if act is None:
+            raise UnsupportedError(f"{name} must be float32, float16 or bfloat16, not {t.dtype}")
+        if t.device.type != "cuda" or t.device.index != self.device:
+            raise ConfigError(f"{name} must be on cuda:{self.device}, not {t.device}")
+        if t.dim() != 3 or t.shape[0] != rows or t.shape[1] != heads or t.shape[2] != hd:
+            raise ShapeError(f"{name} must be {(rows, heads, hd)}, not {tuple(t.shape)}")
+        sr, sh, sd = t.stride()
+        if (hd > 1 and sd != 1) or (heads > 1 and sh != hd):
+            raise UnsupportedError(f"the heads of a {name} row must be contiguous")
+        return act, (sr if rows > 1 else heads * hd)
+
+    def _paged(self, pool, batch):
+        if pool.device != self.device or batch.device != self.device:
+            raise ConfigError(f"page pool and batch must be on cuda:{self.device}")
+        if batch.entries * pool.page_tokens < batch._c.max_kv:
+            raise ShapeError(f"page tables of {batch.entries} entries cannot hold {batch._c.max_kv} tokens")
+
+    def rope_append(self, pool: PagePool, batch: PageBatch, q, k, v, inv_freq=None, attn_factor=1.0,
+                    interleaved=False, out=None):
+        """Rotary positions of the call's rows and their append to the pages (aarh_rope_append): q [rows, n_heads,
+        head_dim] or None, k, v [rows, n_kv_heads, head_dim], whose rows may be apart (views of a fused
+        projection); inv_freq [rot_dim / 2] float64 (None: no rotation).  Returns the rotated queries."""
+        import torch
+        self._paged(pool, batch)
+        n, hd = batch.rows, pool.head_dim
+        act, k_ld = self._act("k", k, n, pool.n_kv_heads, hd)
+        v_act, v_ld = self._act("v", v, n, pool.n_kv_heads, hd)
+        heads = q_ld = o_ld = 0
+        if q is not None:
+            heads = q.shape[1]
+            q_act, q_ld = self._act("q", q, n, heads, hd)
+            if out is None:
+                out = torch.empty((n, heads, hd), dtype=q.dtype, device=q.device)
+            o_act, o_ld = self._act("out", out, n, heads, hd)
+            if q_act != act or o_act != act:
+                raise UnsupportedError("q, k, v and out must have one type")
+        if v_act != act:
+            raise UnsupportedError("q, k, v and out must have one type")
+        f = _on(self.device, "inv_freq", inv_freq, torch.float64, 1)
+        a = _RopeArgs(act, heads, None if q is None else q.data_ptr(), k.data_ptr(), v.data_ptr(), q_ld, k_ld, v_ld,
+                      None if q is None else out.data_ptr(), o_ld, f, 0 if inv_freq is None else 2 * inv_freq.shape[0],
+                      1 if interleaved else 0, attn_factor)
+        st = lib().aarh_rope_append(self.h, pool._c, batch._c, a, _stream(self.device))
+        if st:
+            self._check(st)
+        return out
+
+    def paged_attention(self, pool: PagePool, batch: PageBatch, q, scale=None, softcap=0.0, window=0, slopes=None,
+                        prefix=None, grouped=False, out=None):
+        """Attention of the call's rows q [rows, n_heads, head_dim] over the paged cache (aarh_paged_attention):
+        causal, with an optional tanh cap on the scores, sliding window, distance slope per head [n_heads] f32
+        and bidirectional prefix length per sequence [nseq] int32.  Returns [rows, n_heads, head_dim]."""
+        import torch
+        self._paged(pool, batch)
+        n, hd, heads = batch.rows, pool.head_dim, q.shape[1] if q.dim() == 3 else 0
+        act, q_ld = self._act("q", q, n, heads, hd)
+        if out is None:
+            out = torch.empty((n, heads, hd), dtype=q.dtype, device=q.device)
+        o_act, o_ld = self._act("out", out, n, heads, hd)
+        if o_act != act:
+            raise UnsupportedError("q and out must have one type")
+        sl = _on(self.device, "slopes", slopes, torch.float32, 1)
+        pre = _on(self.device, "prefix", prefix, torch.int32, 1)
+        if (slopes is not None and slopes.shape[0] != heads) or (prefix is not None and prefix.shape[0] != batch._c.nseq):
+            raise ShapeError("slopes has a value for each head, prefix one for each sequence")
+        a = _PagedAttnArgs(act, heads, 1 if grouped else 0, q.data_ptr(), q_ld, out.data_ptr(), o_ld,
+                           hd ** -0.5 if scale is None else scale, softcap, window, sl, pre, None, 0)
+        key = (act, heads, window, pre is None, pool.kv_format, pool.n_kv_heads, hd, pool.page_tokens)
+        need = batch._workspace.get(key)
+        if need is None:
+            size = C.c_int64()
+            self._check(lib().aarh_paged_attention_workspace(self.h, pool._c, batch._c, a, C.byref(size)))
+            need = batch._workspace[key] = size.value
+        if need:
+            ws = torch.empty(need, dtype=torch.uint8, device=q.device)  # the stream's until the call has run
+            a.workspace, a.workspace_bytes = ws.data_ptr(), need
+        st = lib().aarh_paged_attention(self.h, pool._c, batch._c, a,
+                                        _stream(self.device))
+        if st:
+            self._check(st)
+        return out
+
+    def process_logits(self, logits, history=None, history_len=None, prompt_len=None, penalties=None, rows_per_seq=1,
+                       draft=None, bias_off=None, bias_ids=None, bias_vals=None, masks=None, mask_of_row=None,
+                       out=None):
+        """Penalties, biases and grammar masks (aarh_process_logits) on logits [nseq * rows_per_seq, vocab] f32, whose rows may
+        be apart: history [nseq, n] int32 with history_len and prompt_len [nseq], penalties [nseq, 3] f32
+        (repetition, presence, frequency), draft [nseq, rows_per_seq - 1] int32 proposals, biases as bias_off
+        [nseq + 1] into bias_ids / bias_vals, masks [n, ceil(vocab / 32)] int32 bits and mask_of_row.
+        out may be logits (in place).  Returns the processed rows."""
+        import torch
+        if rows_per_seq <= 0 or logits.dim() != 2 or logits.shape[0] % rows_per_seq:
+            raise ShapeError(f"logits {tuple(logits.shape)} are not rows of {rows_per_seq} for each sequence")
+        rows, V = logits.shape
+        n, dev, i32, f32 = rows // rows_per_seq, self.device, torch.int32, torch.float32
+        if out is None:
+            out = torch.empty((rows, V), dtype=f32, device=logits.device)
+        for name, t in (("logits", logits), ("out", out)):
+            _on(dev, name, t, f32, 2, contiguous=False)
+            if tuple(t.shape) != (rows, V) or (V > 1 and t.stride(1) != 1):
+                raise UnsupportedError(f"{name} must be {(rows, V)} with contiguous rows")
+        for name, t, shape in (("history_len", history_len, (n,)), ("prompt_len", prompt_len, (n,)),
+                               ("penalties", penalties, (n, 3)), ("bias_off", bias_off, (n + 1,)),
+                               ("mask_of_row", mask_of_row, (rows,))):
+            if t is not None and tuple(t.shape) != shape:
+                raise ShapeError(f"{name} must be {shape}, not {tuple(t.shape)}")
+        if (history is not None and history.shape[0] != n) or (draft is not None and draft.shape[0] != n):
+            raise ShapeError(f"history and draft must have a row for each of {n} sequences")
+        if draft is not None and draft.shape[1] < rows_per_seq - 1:
+            raise ShapeError(f"{rows_per_seq} rows need {rows_per_seq - 1} proposals, got {draft.shape[1]}")
+        if masks is not None and masks.shape[0] == 0:
+            raise ShapeError("masks is empty")
+        if (bias_ids is None) != (bias_vals is None) or (bias_ids is not None and bias_ids.shape != bias_vals.shape):
+            raise ShapeError("bias_ids and bias_vals must have one length")
+        if bias_off is not None and bias_ids is None:
+            raise ConfigError("bias_off needs bias_ids and bias_vals")
+        a = _LogitsArgs(n, rows_per_seq, V, logits.data_ptr(), logits.stride(0) if rows > 1 else V, out.data_ptr(),
+                        out.stride(0) if rows > 1 else V, _on(dev, "history", history, i32, 2),
+                        0 if history is None else history.shape[1], _on(dev, "history_len", history_len, i32, 1),
+                        _on(dev, "prompt_len", prompt_len, i32, 1), _on(dev, "penalties", penalties, f32, 2),
+                        _on(dev, "draft", draft, i32, 2), 0 if draft is None else draft.shape[1],
+                        _on(dev, "bias_off", bias_off, i32, 1), _on(dev, "bias_ids", bias_ids, i32, 1),
+                        _on(dev, "bias_vals", bias_vals, f32, 1), 0 if bias_ids is None else bias_ids.shape[0],
+                        _on(dev, "masks", masks, i32, 2), 0 if masks is None else masks.shape[1],
+                        0 if masks is None else masks.shape[0], _on(dev, "mask_of_row", mask_of_row, i32, 1))
+        st = lib().aarh_process_logits(self.h, a, _stream(dev))
+        if st:
+            self._check(st)
+        return out
 
 
 class MtpSpeculativeEngine:

@@ -600,8 +600,10 @@ int stage_release(aarh_ctx* c, int slot) {
 }  // namespace
 
 namespace aarh {
-// Records a failure on a context for the library's other translation units (weights.cpp).
+// A context's error text and device for the library's other translation units (weights.cpp,
+// paged_runtime.cpp).
 int ctx_fail(aarh_ctx* c, int code, const char* msg) { return fail(c, code, "%s", msg); }
+int ctx_device(const aarh_ctx* c) { return c->device; }
 // RopeScalingConfig::validate (config.rs:52-96) of a checkpoint config, for weights.cpp.
 int rope_scaling_check(int head_dim, int max_seq_len, const aarh_rope_scaling* s, std::string& err);
 }  // namespace aarh

@@ -559,6 +559,11 @@ namespace aarh {
 int ctx_fail(aarh_ctx* c, int code, const char* msg);
 int lat_ctx_fail(aarh_lat_ctx* c, int code, const char* msg);
 int rope_scaling_check(int head_dim, int max_seq_len, const aarh_rope_scaling* s, std::string& err);
+// Records a failure of a context-free call of another translation unit.
+int host_fail(int code, const char* msg) {
+    g_host_err = msg;
+    return code;
+}
 }  // namespace aarh
 
 namespace {

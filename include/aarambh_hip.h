@@ -354,6 +354,147 @@ int aarh_prof_enable(aarh_ctx *ctx, int enable);
 int aarh_prof_get(aarh_ctx *ctx, int cls, double *total_ms, double *alg_bytes, int64_t *launches);
 
 /* ===================================================================================
+ * Operators over a paged key / value cache, and on logits: DEVICE pointers, any stream.
+ *
+ * A page pool holds the keys and values of many sequences in pages of page_tokens tokens;
+ * a sequence's page table names its pages in order.  A call's new rows (one decode token,
+ * a verify step's k + 1 rows, a prompt chunk) lie one after another in the activation
+ * buffers, sequence after sequence.  These entries allocate nothing and wait for nothing
+ * (they may be captured into a graph); `stream` is a hipStream_t of the context's device,
+ * AARH_DEFAULT_STREAM (that device's default stream) or NULL (the context's stream).  They
+ * touch no state of the context except its error text, and run on its device whichever one
+ * is current.
+ * =================================================================================== */
+#define AARH_DEFAULT_STREAM ((void *)1)
+enum { AARH_A_F32 = 0, AARH_A_F16 = 1, AARH_A_BF16 = 2 }; /* activation element types */
+enum { AARH_KV_BF16 = 3 };                                /* page pools only */
+/* status bits of a sequence: a page table entry that a new or visible token needs is not a
+   page of the pool (such tokens are not stored, and count as absent); row_off / kv_len
+   contradict each other or max_rows / max_kv (the sequence is left out, its rows and pages as they were). */
+enum { AARH_SEQ_BAD_PAGE = 1, AARH_SEQ_BAD_LENGTH = 2 };
+
+/* k, v: [n_pages][n_kv_heads][page_tokens * head_dim] elements of kv_format (AARH_KV_F16,
+   AARH_KV_BF16 or AARH_KV_INT8), 16-byte aligned.  Tokens are kept in blocks of 32, in the order the
+   matrix instructions read them: with t = 8 a + 4 s + b, d = 64 c + 16 g + 8 h + j a block of
+   16-bit keys is [s][c][h][g][a][b][j], of INT8 keys [s][c][g][a][b][h][j]; values are V^T,
+   [d][t], or for INT8, with d = 32 p + 16 h + r and t = 8 g + j, [p][g][r][h][j].  INT8: one fp16 scale per
+   (token, kv head), [n_pages][n_kv_heads][page_tokens]; the value is code * scale. */
+typedef struct {
+    int32_t kv_format, n_kv_heads;
+    int32_t head_dim;    /* 64 or 128 */
+    int32_t page_tokens; /* 32, 64, 128 or 256 */
+    int32_t n_pages;
+    void *k, *v;
+    uint16_t *k_scale, *v_scale; /* INT8 pools */
+} aarh_page_pool;
+
+/* The sequences of one call.  Sequence b's rows are row_off[b] .. row_off[b + 1] - 1 of the
+   activation buffers (any number, also none), the last of its kv_len[b] cached tokens: row i has
+   position kv_len[b] - rows_b + i.  Rows from row_off[nseq] on are left as they were. */
+typedef struct {
+    int32_t nseq;
+    int32_t rows;     /* rows of the activation buffers */
+    int32_t max_rows; /* bound on the rows of a sequence */
+    int32_t max_kv;   /* bound on kv_len */
+    const int32_t *row_off; /* [nseq + 1] */
+    const int32_t *kv_len;  /* [nseq] */
+    const int32_t *tables;  /* [nseq][table_ld] page numbers, table_ld * page_tokens >= max_kv; entries that no
+                               token of the call needs may hold anything */
+    int64_t table_ld;
+    int32_t *status;        /* [nseq] or NULL: AARH_SEQ_* bits are or-ed in (the caller clears them) */
+} aarh_page_batch;
+
+/* --- rotary positions and cache append (RopeCache::apply_rotate, nn/src/rope.rs:17-136, and
+   KVCache::append, nn/src/kvcache.rs:265-368, for pages).  Rotates the first rot_dim dimensions of every
+   head of q and k by position * inv_freq[i] (angles in f64): pairs (i, i + rot_dim / 2), or
+   (2 i, 2 i + 1) with interleaved = 1; cos and sin are multiplied by attn_factor, the other dimensions
+   pass unchanged.  Writes the queries to q_out (may be q) and keys and values to the pages
+   of their positions; INT8 pools: absmax scale per (token, kv head), as the context's INT8 cache.
+   Rows are *_ld elements apart, heads head_dim elements; every pointer 16-byte aligned and every
+   *_ld a multiple of 16 bytes (UNSUPPORTED otherwise).  rot_dim: a multiple of 16 up to head_dim, or 0 (q is
+   copied, inv_freq may be NULL).  act F32 with F16 or INT8 pools, F16 with F16 or INT8, BF16 with BF16. --- */
+typedef struct {
+    int32_t act, n_heads; /* n_heads: query heads, 0 = no queries (keys and values only) */
+    const void *q, *k, *v;
+    int64_t q_ld, k_ld, v_ld;
+    void *q_out;
+    int64_t q_out_ld;
+    const double *inv_freq; /* [rot_dim / 2] */
+    int32_t rot_dim, interleaved;
+    float attn_factor;
+} aarh_rope_args;
+int aarh_rope_append(aarh_ctx *ctx, const aarh_page_pool *pool, const aarh_page_batch *batch,
+                     const aarh_rope_args *args, void *stream);
+/* inv_freq [rot_dim / 2] and the cos / sin factor of a scaling (NULL: none) in f64, by the formulas of
+   aarh_set_rope_scaling, for aarh_rope_append (host memory; message in aarh_host_last_error). */
+int aarh_rope_frequencies(int32_t rot_dim, double theta, int32_t max_seq_len, const aarh_rope_scaling *scaling,
+                          double *inv_freq, float *attn_factor);
+
+/* --- attention of the call's rows over the paged cache (GroupedQueryAttention::forward,
+   nn/src/attention.rs:170-222; causal with shift kv_len - rows), after aarh_rope_append.
+   score = scale q.k; softcap > 0: softcap tanh(score / softcap); slopes: + slopes[head] (j - p) for
+   key j and row position p.  Key j < kv_len is visible if j <= p and (window = 0 or p - j < window),
+   or if j < prefix[b].  out = softmax(score) v over the visible keys, zero where there are none.
+   Query head h reads kv head h % n_kv_heads (the reference's map), or h / (n_heads /
+   n_kv_heads) with grouped = 1.  Types as for aarh_rope_append; out has q's type.  A key that no row
+   of a call sees may hold anything; one that some row sees must be finite.
+   workspace: aarh_paged_attention_workspace bytes (16-byte aligned; may be NULL when that is 0),
+   used by this call alone until it has run. --- */
+typedef struct {
+    int32_t act, n_heads, grouped;
+    const void *q; /* [rows][q_ld] */
+    int64_t q_ld;
+    void *out;     /* [rows][out_ld], not overlapping q */
+    int64_t out_ld;
+    float scale, softcap;
+    int32_t window;
+    const float *slopes;   /* [n_heads] or NULL */
+    const int32_t *prefix; /* [nseq] or NULL */
+    void *workspace;
+    int64_t workspace_bytes;
+} aarh_paged_attn_args;
+int aarh_paged_attention(aarh_ctx *ctx, const aarh_page_pool *pool, const aarh_page_batch *batch,
+                         const aarh_paged_attn_args *args, void *stream);
+/* Bytes of workspace that the call needs: of the shapes alone (nseq, max_rows, max_kv, heads,
+   window and whether there is a prefix); no pointer is read. */
+int aarh_paged_attention_workspace(aarh_ctx *ctx, const aarh_page_pool *pool, const aarh_page_batch *batch,
+                                   const aarh_paged_attn_args *args, int64_t *bytes);
+
+/* --- penalties, biases and grammar masks on logits, before aarh_accept_sample and
+   aarh_top_candidates (constrained_distribution, inference/src/speculative.rs:629-664).
+   Row b * rows_per_seq + t holds sequence b's logits after its history and its first t proposals.
+   With c = how often a token stands in history[prompt_len ..] and those proposals, and `seen` = c > 0
+   or in history[.. prompt_len]:  x = x > 0 ? x / repetition : x * repetition where seen;
+   x -= presence where c > 0;  x -= frequency * c;  x += the token's bias;  -inf where the row's mask
+   has bit 0.  A bias list that names a token twice uses its last value; ids from vocab on in
+   histories, proposals and bias lists are ignored; lengths are cut to what the arrays hold. --- */
+typedef struct {
+    int32_t nseq, rows_per_seq, vocab;
+    const float *logits; /* [nseq * rows_per_seq][ld] */
+    int64_t ld;
+    float *out;          /* [nseq * rows_per_seq][out_ld]; may be logits (with out_ld = ld) */
+    int64_t out_ld;
+    const uint32_t *history; /* [nseq][history_ld], NULL: none */
+    int64_t history_ld;
+    const int32_t *history_len; /* [nseq] */
+    const int32_t *prompt_len;  /* [nseq], NULL: 0 */
+    const float *penalties;     /* [nseq][3] repetition (> 0), presence, frequency; NULL: none */
+    const uint32_t *draft;      /* [nseq][draft_ld >= rows_per_seq - 1], NULL: none */
+    int64_t draft_ld;
+    const int32_t *bias_off;    /* [nseq + 1] into the next two, NULL: none */
+    const uint32_t *bias_ids;
+    const float *bias_vals;
+    int32_t n_bias;             /* their length */
+    const uint32_t *masks;      /* [n_masks][mask_ld >= ceil(vocab / 32)] bit v % 32 of word v / 32: token v may
+                                   follow; NULL: none */
+    int64_t mask_ld;
+    int32_t n_masks;
+    const int32_t *mask_of_row; /* [nseq * rows_per_seq] mask of each row, -1 none (any other number
+                                   that is no mask: every token masked) */
+} aarh_logits_args;
+int aarh_process_logits(aarh_ctx *ctx, const aarh_logits_args *args, void *stream);
+
+/* ===================================================================================
  * Latent-attention MoE decoder (benchmark config 5): blocks of multi-head latent
  * attention (nn/src/mla.rs:300-489, built by model/src/model.rs:1094-1156) and a
  * fine-grained MoE FFN with top-k routing and shared experts (nn/src/moe.rs:127-406).
