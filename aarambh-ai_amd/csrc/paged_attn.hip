@@ -1,7 +1,18 @@
 // Attention of a call's new rows over the paged key / value cache.
 //
-// One wave per (row, query head): 64 keys at a time, one a lane, with the running maximum and sum
-// of the softmax; then each lane adds its output dimensions over the 64 keys.
+// Rows of one sequence that read one kv head (its `group` query heads, token by token: row r is query head
+// r % group of new token r / group) form the columns of S^T = K Q^T and O^T = V^T P^T.  In the matrix instructions'
+// result layout a lane then holds the scores of ONE query for eight consecutive tokens, which is
+// the operand layout of P^T: the softmax needs no exchange but a maximum over the four 16-lane
+// rows of the wave, P never leaves the registers, and O's columns take the running factor lane by lane.
+// The pages store K and V in operand order, so a wave's load is 1 KiB of consecutive bytes.
+//
+// Running maximum, sum and O are f32.  P is rounded to the pool's 16 bits for the product with V
+// (2^-11 or 2^-8 of each weight, as V itself was); f32 queries are split into fp16 hi + lo
+// halves, and so is P (2^-22 together): two matrix instructions in place of one.
+#include <algorithm>
+#include <type_traits>
+
 #include "device_common.hpp"
 #include "paged.hpp"
 
@@ -9,99 +20,514 @@ namespace aarh {
 
 namespace {
 
-template <typename T, typename C, bool I8, int HD>
-__global__ __launch_bounds__(64) void paged_attn_kernel(PagedAttnArgs a) {
-    const int lane = threadIdx.x, i = blockIdx.x, h = blockIdx.y, b = blockIdx.z;
-    __shared__ float s_q[HD], s_p[64];
-    PageSeq s;
-    if (!page_seq(a.bt.row_off, a.bt.kv_len, b, a.bt.rows, a.bt.max_rows, a.bt.max_kv, &s)) {
-        if (a.bt.status && lane == 0) atomicOr(&a.bt.status[b], PAGE_SEQ_BAD_LENGTH);
-        return;
-    }
-    if (i >= s.rows) return;
-    const int p = s.kv_len - s.rows + i;
-    const int kvh = a.grouped ? h / (a.n_heads / a.pool.n_kv) : h % a.pool.n_kv;
-    const int pre = a.prefix ? min(a.prefix[b], s.kv_len) : 0;
-    const T* q = (const T*)a.q + (long long)(s.row0 + i) * a.q_ld + h * HD;
-    for (int d = lane; d < HD; d += 64) s_q[d] = (float)q[d];
-    const float slope = a.slopes ? a.slopes[h] : 0.f;
-    const int low = a.window ? max(0, p - a.window + 1) : 0;
-    const int end = max(p + 1, pre);
-    float m = -INFINITY, l = 0.f, o[HD / 64] = {};
-    bool bad = false;
-    const int32_t* table = a.bt.tables + b * a.bt.table_ld;
-    for (int t0 = 0; t0 < end; t0 += 64) {
-        if (t0 >= pre && t0 + 64 <= low) continue;
-        const int t = t0 + lane;
-        const bool vis = t < end && ((t <= p && t >= low) || t < pre);
-        int page = -1;
-        if (vis) {
-            page = page_of(table, t, a.pool.page_shift, a.pool.n_pages);
-            bad |= page < 0;
-        }
-        const int in_page = t & ((1 << a.pool.page_shift) - 1);
-        const size_t head = (size_t)max(page, 0) * a.pool.n_kv + kvh;
-        const size_t base = (head << a.pool.page_shift) * HD + (size_t)(in_page >> 5) * (PAGE_BLK * HD);
-        const size_t tok = (head << a.pool.page_shift) + in_page;
-        float x = -INFINITY, vsc = 0.f;
-        __syncthreads();
-        if (page >= 0) {
-            x = 0.f;
-            for (int d = 0; d < HD; d++) x += s_q[d] * (float)((const C*)a.pool.k)[base + page_k_at(t & 31, d, HD, I8)];
-            if (I8) {
-                x *= (float)__builtin_bit_cast(_Float16, a.pool.ks[tok]);
-                vsc = (float)__builtin_bit_cast(_Float16, a.pool.vs[tok]);
-            }
-            x *= a.scale;
-            if (a.softcap > 0.f) x = a.softcap * tanhf(x / a.softcap);
-            x += slope * (float)(t - p);
-        }
-        const float mx = fmaxf(m, wave_max_f32(x));
-        const float use = mx == -INFINITY ? 0.f : mx;
-        const float e = __expf(x - use), alpha = __expf(m - use);
-        l = l * alpha + wave_sum_f32(e);
-        m = mx;
-        s_p[lane] = I8 ? e * vsc : e;
-        __syncthreads();
-        for (int k = 0; k < HD / 64; k++) o[k] *= alpha;
-        for (int j = 0; j < 64; j++) {
-            const unsigned at_lo = __builtin_amdgcn_readlane((int)(uint32_t)base, j);
-            const unsigned at_hi = __builtin_amdgcn_readlane((int)(uint32_t)(base >> 32), j);
-            const size_t at = ((size_t)at_hi << 32) | at_lo;
-            const int pg = __builtin_amdgcn_readlane(page, j);
-            if (pg < 0) continue;
-            for (int k = 0; k < HD / 64; k++)
-                o[k] += s_p[j] * (float)((const C*)a.pool.v)[at + page_v_at((t0 + j) & 31, lane + 64 * k, HD, I8)];
-        }
-    }
-    T* out = (T*)a.out + (long long)(s.row0 + i) * a.out_ld + h * HD;
-    const float inv = l > 0.f ? 1.f / l : 0.f;
-    for (int k = 0; k < HD / 64; k++) out[lane + 64 * k] = (T)(o[k] * inv);
-    if (bad && a.bt.status) atomicOr(&a.bt.status[b], PAGE_SEQ_BAD_PAGE);
+typedef __bf16 bfrag_t __attribute__((ext_vector_type(8)));
+typedef unsigned u32x4_t __attribute__((ext_vector_type(4)));
+
+constexpr float PA_LOG2E = 1.4426950408889634f;
+
+// Element type of the matrix instructions for a pool format.
+template <int KVF>
+struct Mat {
+    typedef typename std::conditional<KVF == KV_BF16, bfrag_t, half8_t>::type frag;
+    typedef typename std::conditional<KVF == KV_BF16, __bf16, _Float16>::type elem;
+    // fp16 weights are scaled by 2^14 (a power of two in the exponent's argument, cancelled by the sum): the
+    // smallest steps of fp16 are then 2^-38 of the largest weight
+    static constexpr float P_BITS = KVF == KV_BF16 ? 0.f : 14.f;
+};
+
+template <int KVF>
+__device__ __forceinline__ float4_t mfma16(typename Mat<KVF>::frag a, typename Mat<KVF>::frag b, float4_t c) {
+    if constexpr (KVF == KV_BF16) return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
+    else return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
 }
 
-template <typename T, typename C, bool I8>
+// 8 INT8 codes as fp16, exactly: code + 128 in the mantissa of 1024, minus 1152
+__device__ __forceinline__ half8_t i8_to_half8(uint32_t d0, uint32_t d1) {
+    typedef _Float16 half2v __attribute__((ext_vector_type(2)));
+    const half2v off = {(_Float16)1152.f, (_Float16)1152.f};
+    d0 ^= 0x80808080u;
+    d1 ^= 0x80808080u;
+    union {
+        half8_t h;
+        half2v p[4];
+    } r;
+    r.p[0] = __builtin_bit_cast(half2v, __builtin_amdgcn_perm(0x64646464u, d0, 0x04010400u)) - off;
+    r.p[1] = __builtin_bit_cast(half2v, __builtin_amdgcn_perm(0x64646464u, d0, 0x04030402u)) - off;
+    r.p[2] = __builtin_bit_cast(half2v, __builtin_amdgcn_perm(0x64646464u, d1, 0x04010400u)) - off;
+    r.p[3] = __builtin_bit_cast(half2v, __builtin_amdgcn_perm(0x64646464u, d1, 0x04030402u)) - off;
+    return r.h;
+}
+
+__device__ __forceinline__ float row16_max(float x) {
+    auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    x = fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
+    auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
+}
+__device__ __forceinline__ float row16_sum(float x) {
+    auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    x = __uint_as_float(a[0]) + __uint_as_float(a[1]);
+    auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return __uint_as_float(b[0]) + __uint_as_float(b[1]);
+}
+
+// tanh to a few units: a series where the quotient would cancel
+__device__ __forceinline__ float tanh_f32(float x) {
+    const float y = fabsf(x), y2 = y * y;
+    const float series = y * (1.f + y2 * (-0.33333333333f + y2 * (0.13333333333f + y2 * (-0.053968253968f + y2 * (0.021869488536f - y2 * 0.0088632355299f)))));
+    const float e = __builtin_amdgcn_exp2f(y * (2.f * PA_LOG2E));
+    const float big = 1.f - 2.f / (e + 1.f);
+    return copysignf(y < 0.3f ? series : big, x);
+}
+
+// What a tile of query rows needs to know of its sequence.
+struct TileInfo {
+    PageSeq s;
+    int b, kvh, r0;        // first row (token x group member) of the tile
+    int p_lo, p_hi, pre;   // positions of its first and last rows; prefix length
+    int low;               // first key that the window leaves to any row
+    int pre_blk, lo_blk, n;  // 32-token blocks it visits: 0 .. pre_blk - 1, then lo_blk ..; n in all
+};
+
+// Blocks of a tile: those of the prefix that lie before the window, then from the window's start to
+// the last visible key.
+__device__ __forceinline__ bool tile_info(const PagedAttnArgs& a, int b, int kvh, int tile, int tile_rows, int group, TileInfo* t) {
+    if (!page_seq(a.bt.row_off, a.bt.kv_len, b, a.bt.rows, a.bt.max_rows, a.bt.max_kv, &t->s)) {
+        if (a.bt.status && threadIdx.x == 0) atomicOr(&a.bt.status[b], PAGE_SEQ_BAD_LENGTH);
+        return false;
+    }
+    t->b = b;
+    t->kvh = kvh;
+    t->r0 = tile * tile_rows;
+    const int rows = t->s.rows * group;
+    if (t->r0 >= rows) return false;
+    const int pos0 = t->s.kv_len - t->s.rows;
+    t->p_lo = pos0 + t->r0 / group;
+    t->p_hi = pos0 + (min(t->r0 + tile_rows, rows) - 1) / group;
+    t->pre = a.prefix ? min(max(a.prefix[b], 0), t->s.kv_len) : 0;
+    t->low = a.window ? max(0, t->p_lo - a.window + 1) : 0;
+    t->lo_blk = t->low >> 5;
+    t->pre_blk = min((t->pre + 31) >> 5, t->lo_blk);
+    t->n = t->pre_blk + ((max(t->p_hi + 1, t->pre) + 31) >> 5) - t->lo_blk;
+    return true;
+}
+
+__device__ __forceinline__ int tile_block(const TileInfo& t, int k) { return k < t.pre_blk ? k : t.lo_blk + (k - t.pre_blk); }
+
+__device__ __forceinline__ int head_of(const PagedAttnArgs& a, int kvh, int m, int group) {
+    return a.grouped ? kvh * group + m : m * a.pool.n_kv + kvh;
+}
+
+// Workspace of a call split over the keys: [split][row x head][hd] weighted sums, then their (maximum, sum).
+__device__ __forceinline__ float* part_o(const PagedAttnArgs& a, int split, long long slot) {
+    return (float*)a.workspace + ((long long)split * a.bt.rows * a.n_heads + slot) * a.pool.hd;
+}
+__device__ __forceinline__ float2_t* part_ml(const PagedAttnArgs& a, int splits, int split, long long slot) {
+    const long long slots = (long long)a.bt.rows * a.n_heads;
+    return (float2_t*)((float*)a.workspace + splits * slots * a.pool.hd) + split * slots + slot;
+}
+
+// ---------------------------------------------------------------------------
+// Few rows: the cache is streamed through the registers
+// ---------------------------------------------------------------------------
+constexpr int DC_WAVES = 4;
+
+template <typename T, int KVF, int HD, int NT>
+__global__ __launch_bounds__(DC_WAVES * 64, 2) void paged_decode_kernel(PagedAttnArgs a, int group, int tiles, int splits, int per) {
+    typedef typename Mat<KVF>::frag frag;
+    typedef typename Mat<KVF>::elem elem;
+    constexpr bool I8 = KVF == KV_INT8, F32 = std::is_same<T, float>::value;
+    constexpr int KS = HD / 32;              // k-steps of K Q^T
+    constexpr int DT = HD / 16;              // 16-dimension tiles of O^T
+    constexpr int KL = I8 ? HD / 32 : HD / 16;  // 16-byte pieces of a lane's share of a K (or V) block
+    constexpr int BLK = PAGE_BLK * HD * (I8 ? 1 : 2);
+    constexpr int LDO = HD + 4;
+    __shared__ float s_o[DC_WAVES][16 * LDO];
+    __shared__ float2_t s_ml[DC_WAVES][16];
+    const int tid = threadIdx.x, lane = tid & 63, wid = __builtin_amdgcn_readfirstlane(tid >> 6), lr = lane & 15, lg = lane >> 4;
+    // workgroup -> (pair of sequence and kv head, tile, split), pairs fastest
+    int id = blockIdx.x;
+    const int pairs = a.bt.nseq * a.pool.n_kv;
+    const int pair = id % pairs;
+    id /= pairs;
+    const int tile = id % tiles, split = id / tiles;
+    TileInfo t;
+    if (!tile_info(a, pair / a.pool.n_kv, pair % a.pool.n_kv, tile, 16 * NT, group, &t)) return;
+    const int k0 = split * per, k1 = min(k0 + per, t.n);
+    const int rows = t.s.rows * group, pos0 = t.s.kv_len - t.s.rows;
+
+    // this lane's queries: columns lr of NT tiles
+    frag qh[NT][KS], ql[NT][F32 ? KS : 1];
+    float qs[NT], slope[NT];
+    int pos[NT];
+#pragma unroll
+    for (int nt = 0; nt < NT; nt++) {
+        const int r = t.r0 + nt * 16 + lr, rr = min(r, rows - 1), tok = rr / group;
+        const int h = head_of(a, t.kvh, rr - tok * group, group);
+        pos[nt] = r < rows ? pos0 + tok : -1;  // -1: a column of no row, sees at most prefix keys
+        slope[nt] = a.slopes ? a.slopes[h] * PA_LOG2E : 0.f;
+        const T* q = (const T*)a.q + (long long)(t.s.row0 + tok) * a.q_ld + (long long)h * HD + 16 * lg;
+        qs[nt] = a.scale;
+        if constexpr (F32) {
+            float x[KS][8], top = 0.f;
+#pragma unroll
+            for (int ks = 0; ks < KS; ks++) {
+                const float* src = q + 64 * (ks >> 1) + 8 * (ks & 1);
+                const float4_t u = *(const float4_t*)src, v = *(const float4_t*)(src + 4);
+#pragma unroll
+                for (int j = 0; j < 4; j++) {
+                    x[ks][j] = u[j];
+                    x[ks][4 + j] = v[j];
+                }
+#pragma unroll
+                for (int j = 0; j < 8; j++) top = fmaxf(top, fabsf(x[ks][j]));
+            }
+            // a power of two brings the row's largest value to [1/2, 1) (fp16's range); the scale takes it back
+            const int e = __builtin_amdgcn_frexp_expf(row16_max(top));
+            const float inv = ldexpf(1.f, -max(e, -120));
+            qs[nt] = ldexpf(a.scale, max(e, -120));
+#pragma unroll
+            for (int ks = 0; ks < KS; ks++)
+#pragma unroll
+                for (int j = 0; j < 8; j++) {
+                    const float v = x[ks][j] * inv;
+                    qh[nt][ks][j] = (_Float16)v;
+                    ql[nt][ks][j] = (_Float16)(v - (float)qh[nt][ks][j]);
+                }
+        } else {
+#pragma unroll
+            for (int ks = 0; ks < KS; ks++) {
+                if constexpr (std::is_same<T, elem>::value) qh[nt][ks] = *(const frag*)(q + 64 * (ks >> 1) + 8 * (ks & 1));
+            }
+        }
+    }
+
+    float m[NT], l[NT];
+    float4_t o[NT][DT];
+#pragma unroll
+    for (int nt = 0; nt < NT; nt++) {
+        m[nt] = -INFINITY;
+        l[nt] = 0.f;
+#pragma unroll
+        for (int d = 0; d < DT; d++) o[nt][d] = float4_t{0.f, 0.f, 0.f, 0.f};
+    }
+
+    const int32_t* table = a.bt.tables + t.b * a.bt.table_ld;
+    const int shift = a.pool.page_shift - 5;  // blocks of a page
+    const bool plain = a.softcap == 0.f && a.slopes == nullptr;
+    u32x4_t kr[KL], vr[KL], ksc, vsc;
+    // this wave's blocks: k0 + wid, k0 + wid + DC_WAVES, ..
+    auto page_at = [&](int k) __attribute__((always_inline)) {
+        const int blk = tile_block(t, k);
+        return table[blk >> shift];
+    };
+    size_t off = 0;  // element offset of the block in K and V
+    auto locate = [&](int k, int page) __attribute__((always_inline)) {
+        const int blk = tile_block(t, k);
+        const int p = page >= 0 && page < a.pool.n_pages ? page : 0;
+        off = ((((size_t)p * a.pool.n_kv + t.kvh) << shift) + (blk & ((1 << shift) - 1))) * PAGE_BLK;
+    };
+    auto load_k = [&]() __attribute__((always_inline)) {
+        const char* p = (const char*)a.pool.k + off * (BLK / PAGE_BLK) + lane * 16;
+#pragma unroll
+        for (int i = 0; i < KL; i++) kr[i] = __builtin_nontemporal_load((const u32x4_t*)(p + i * 1024));
+        if constexpr (I8) ksc = *(const u32x4_t*)(a.pool.ks + off + 8 * lg);
+    };
+    auto load_v = [&]() __attribute__((always_inline)) {
+        const char* p = (const char*)a.pool.v + off * (BLK / PAGE_BLK) + (I8 ? lane : lr * 4 + lg) * 16;
+#pragma unroll
+        for (int i = 0; i < KL; i++) vr[i] = __builtin_nontemporal_load((const u32x4_t*)(p + i * 1024));
+        if constexpr (I8) vsc = *(const u32x4_t*)(a.pool.vs + off + 8 * lg);
+    };
+    auto sc_at = [](u32x4_t s, int i) __attribute__((always_inline)) {
+        const uint32_t w = s[i >> 1];
+        return (float)__builtin_bit_cast(_Float16, (uint16_t)(i & 1 ? w >> 16 : w & 0xFFFFu));
+    };
+    bool bad = false;
+    int k = k0 + wid;
+    int page = 0, page_next = 0;
+    if (k < k1) {
+        page = page_at(k);
+        page_next = page_at(min(k + DC_WAVES, k1 - 1));
+        locate(k, page);
+        load_k();
+        load_v();
+    }
+    for (; k < k1; k += DC_WAVES) {
+        const int t0 = tile_block(t, k) * PAGE_BLK;
+        const bool absent = page < 0 || page >= a.pool.n_pages;
+        bad |= absent;
+        const int kn = k + DC_WAVES;
+        // scores: S^T of tokens 8 lg + 4 ts + i
+        float4_t s[NT][2];
+#pragma unroll
+        for (int nt = 0; nt < NT; nt++) s[nt][0] = s[nt][1] = float4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int ts = 0; ts < 2; ts++)
+#pragma unroll
+            for (int ks = 0; ks < KS; ks++) {
+                frag ka;
+                if constexpr (I8) {
+                    const u32x4_t w = kr[ts * (KS / 2) + (ks >> 1)];
+                    ka = ks & 1 ? i8_to_half8(w[2], w[3]) : i8_to_half8(w[0], w[1]);
+                } else {
+                    ka = __builtin_bit_cast(frag, kr[ts * KS + ks]);
+                }
+#pragma unroll
+                for (int nt = 0; nt < NT; nt++) {
+                    s[nt][ts] = mfma16<KVF>(ka, qh[nt][ks], s[nt][ts]);
+                    if constexpr (F32) s[nt][ts] = mfma16<KVF>(ka, ql[nt][ks], s[nt][ts]);
+                }
+            }
+        const u32x4_t ksc_now = ksc;
+        if (kn < k1) {
+            locate(kn, page_next);
+            load_k();
+        }
+        // visible to every row of the tile: no masks
+        const bool whole = !absent && t0 + PAGE_BLK - 1 <= t.p_lo && (a.window == 0 || t0 > t.p_hi - a.window || t0 + PAGE_BLK <= t.pre);
+        float vexp = 0.f;
+        if constexpr (I8) {
+            // INT8: a weight is multiplied by its token's V scale before it is rounded to fp16, so
+            // the reference of the exponents rises by the exponent of the block's largest scale
+            float top = 0.f;
+#pragma unroll
+            for (int i = 0; i < 8; i++) {
+                const int tok = t0 + 8 * lg + i;
+                const float v = sc_at(vsc, i);
+                top = fmaxf(top, tok < t.s.kv_len ? v : 0.f);
+            }
+            top = row16_max(top);
+            vexp = top > 0x1p-20f ? (float)__builtin_amdgcn_frexp_expf(top) : -20.f;
+        }
+        frag ph[NT], pl[F32 ? NT : 1];
+#pragma unroll
+        for (int nt = 0; nt < NT; nt++) {
+            float x[8];
+#pragma unroll
+            for (int i = 0; i < 8; i++) {
+                x[i] = s[nt][i >> 2][i & 3];
+                if constexpr (I8) x[i] *= sc_at(ksc_now, i);
+            }
+            if (plain) {
+                const float c = qs[nt] * PA_LOG2E;
+#pragma unroll
+                for (int i = 0; i < 8; i++) x[i] *= c;
+            } else {
+#pragma unroll
+                for (int i = 0; i < 8; i++) {
+                    x[i] *= qs[nt];
+                    if (a.softcap > 0.f) x[i] = a.softcap * tanh_f32(x[i] / a.softcap);
+                    x[i] = x[i] * PA_LOG2E + slope[nt] * (float)(t0 + 8 * lg + i - pos[nt]);
+                }
+            }
+            if (!whole) {
+#pragma unroll
+                for (int i = 0; i < 8; i++) {
+                    const int tok = t0 + 8 * lg + i;
+                    const bool seen = !absent && ((tok <= pos[nt] && (a.window == 0 || pos[nt] - tok < a.window)) || tok < t.pre);
+                    x[i] = seen ? x[i] : -INFINITY;
+                }
+            }
+            float mx = x[0];
+#pragma unroll
+            for (int i = 1; i < 8; i++) mx = fmaxf(mx, x[i]);
+            mx = row16_max(mx);
+            if constexpr (I8) mx += vexp;
+            const float mn = fmaxf(m[nt], mx);
+            // rescale only when some column's maximum moved
+            if (__any(mn > m[nt])) {
+                const float alpha = mn == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m[nt] - mn);
+                l[nt] *= alpha;
+#pragma unroll
+                for (int d = 0; d < DT; d++) o[nt][d] *= alpha;
+                m[nt] = mn;
+            }
+            const float ref = (mn == -INFINITY ? 0.f : mn) - Mat<KVF>::P_BITS;
+            float p[8];
+#pragma unroll
+            for (int i = 0; i < 8; i++) {
+                p[i] = __builtin_amdgcn_exp2f(x[i] - ref);
+                l[nt] += p[i];
+                if constexpr (I8) p[i] = x[i] == -INFINITY ? 0.f : p[i] * sc_at(vsc, i);
+            }
+#pragma unroll
+            for (int i = 0; i < 8; i++) {
+                ph[nt][i] = (elem)p[i];
+                if constexpr (F32) pl[nt][i] = (elem)(p[i] - (float)ph[nt][i]);
+            }
+        }
+        // tokens that no row sees may hold anything, also NaN: their V is taken as zero
+        if constexpr (!I8) {
+            if (!whole) {
+                u32x4_t keep;
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    uint32_t w = 0;
+#pragma unroll
+                    for (int e = 0; e < 2; e++) {
+                        const int tok = t0 + 8 * lg + 2 * i + e;
+                        const bool any = (tok <= t.p_hi && tok >= t.low) || tok < t.pre;
+                        w |= any && !absent ? 0xFFFFu << (16 * e) : 0u;
+                    }
+                    keep[i] = w;
+                }
+#pragma unroll
+                for (int i = 0; i < KL; i++) vr[i] &= keep;
+            }
+        }
+#pragma unroll
+        for (int d = 0; d < DT; d++) {
+            frag va;
+            if constexpr (I8) {
+                const u32x4_t w = vr[d >> 1];
+                va = d & 1 ? i8_to_half8(w[2], w[3]) : i8_to_half8(w[0], w[1]);
+            } else {
+                va = __builtin_bit_cast(frag, vr[d]);
+            }
+#pragma unroll
+            for (int nt = 0; nt < NT; nt++) {
+                o[nt][d] = mfma16<KVF>(va, ph[nt], o[nt][d]);
+                if constexpr (F32) o[nt][d] = mfma16<KVF>(va, pl[nt], o[nt][d]);
+            }
+        }
+        if (kn < k1) {
+            load_v();
+            page = page_next;
+            page_next = page_at(min(kn + DC_WAVES, k1 - 1));
+        }
+    }
+    if (bad && a.bt.status && lane == 0) atomicOr(&a.bt.status[t.b], PAGE_SEQ_BAD_PAGE);
+
+    // the waves' shares of each column: joined through LDS
+#pragma unroll
+    for (int nt = 0; nt < NT; nt++) {
+        const float lsum = row16_sum(l[nt]);
+        if (nt) __syncthreads();
+        if (lane < 16) s_ml[wid][lr] = float2_t{m[nt], lsum};
+#pragma unroll
+        for (int d = 0; d < DT; d++) *(float4_t*)&s_o[wid][lr * LDO + 16 * d + 4 * lg] = o[nt][d];
+        __syncthreads();
+        for (int i = tid; i < 16 * (HD / 4); i += DC_WAVES * 64) {
+            const int c = i / (HD / 4), d = i % (HD / 4) * 4;
+            const int r = t.r0 + nt * 16 + c;
+            if (r >= rows) continue;
+            float M = s_ml[0][c][0];
+#pragma unroll
+            for (int w = 1; w < DC_WAVES; w++) M = fmaxf(M, s_ml[w][c][0]);
+            float L = 0.f;
+            float4_t acc = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int w = 0; w < DC_WAVES; w++) {
+                const float2_t ml = s_ml[w][c];
+                const float f = ml[0] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(ml[0] - M);
+                L += ml[1] * f;
+                acc += *(const float4_t*)&s_o[w][c * LDO + d] * f;
+            }
+            const int tok = r / group, h = head_of(a, t.kvh, r - tok * group, group);
+            if (splits > 1) {
+                const long long slot = (long long)(t.s.row0 + tok) * a.n_heads + h;
+                *(float4_t*)(part_o(a, split, slot) + d) = acc;
+                if (d == 0) *part_ml(a, splits, split, slot) = float2_t{M, L};
+            } else {
+                const float inv = L > 0.f ? 1.f / L : 0.f;
+                T* out = (T*)a.out + (long long)(t.s.row0 + tok) * a.out_ld + (long long)h * HD + d;
+#pragma unroll
+                for (int j = 0; j < 4; j++) out[j] = (T)(acc[j] * inv);
+            }
+        }
+    }
+}
+
+// Joins the splits of a call: HD / 4 threads per (row, head).
+template <typename T, int HD>
+__global__ __launch_bounds__(256) void paged_merge_kernel(PagedAttnArgs a, int splits) {
+    const int b = blockIdx.y;
+    PageSeq s;
+    if (!page_seq(a.bt.row_off, a.bt.kv_len, b, a.bt.rows, a.bt.max_rows, a.bt.max_kv, &s)) return;
+    const long long i = (long long)blockIdx.x * 256 + threadIdx.x;
+    const long long at = i / (HD / 4);
+    const int d = (int)(i % (HD / 4)) * 4;
+    if (at >= (long long)s.rows * a.n_heads) return;
+    const long long slot = (long long)s.row0 * a.n_heads + at;
+    float M = -INFINITY;
+    for (int k = 0; k < splits; k++) M = fmaxf(M, (*part_ml(a, splits, k, slot))[0]);
+    float L = 0.f;
+    float4_t acc = {0.f, 0.f, 0.f, 0.f};
+    for (int k = 0; k < splits; k++) {
+        const float2_t ml = *part_ml(a, splits, k, slot);
+        const float f = ml[0] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(ml[0] - M);
+        L += ml[1] * f;
+        acc += *(const float4_t*)(part_o(a, k, slot) + d) * f;
+    }
+    const float inv = L > 0.f ? 1.f / L : 0.f;
+    T* out = (T*)a.out + (s.row0 + at / a.n_heads) * a.out_ld + (at % a.n_heads) * HD + d;
+#pragma unroll
+    for (int j = 0; j < 4; j++) out[j] = (T)(acc[j] * inv);
+}
+
+// ---------------------------------------------------------------------------
+// launch plan
+// ---------------------------------------------------------------------------
+struct Plan {
+    int nt, tiles, splits, per;  // 16-row column tiles of a workgroup, tiles of a (sequence, kv head), splits, blocks each
+};
+
+Plan plan_of(const PagedAttnArgs& a) {
+    const int group = a.n_heads / a.pool.n_kv;
+    const long long rows = (long long)a.bt.max_rows * group;
+    Plan p{};
+    p.nt = rows <= 16 ? 1 : 2;
+    p.tiles = (int)((rows + 16 * p.nt - 1) / (16 * p.nt));
+    // blocks that a tile can visit
+    const int all = (a.bt.max_kv + 31) / 32;
+    const int span = (16 * p.nt + group - 1) / group + 1;
+    const int n = a.window && !a.prefix ? std::min<long long>(all, ((long long)a.window + span) / 32 + 2) : all;
+    // two workgroups per compute unit; a wave gets at least two blocks
+    const long long base = (long long)a.bt.nseq * a.pool.n_kv * p.tiles;
+    const int want = (int)std::max<long long>(1, (512 + base - 1) / base);
+    p.splits = std::max(1, std::min(want, n / (2 * DC_WAVES)));
+    p.per = (n + p.splits - 1) / p.splits;
+    p.per = (p.per + DC_WAVES - 1) / DC_WAVES * DC_WAVES;
+    p.splits = std::max(1, (n + p.per - 1) / p.per);
+    return p;
+}
+
+template <typename T, int KVF, int HD>
 int launch_hd(const PagedAttnArgs& a, hipStream_t stream) {
-    const dim3 grid(a.bt.max_rows, a.n_heads, a.bt.nseq);
-    if (a.pool.hd == 128)
-        hipLaunchKernelGGL((paged_attn_kernel<T, C, I8, 128>), grid, dim3(64), 0, stream, a);
-    else
-        hipLaunchKernelGGL((paged_attn_kernel<T, C, I8, 64>), grid, dim3(64), 0, stream, a);
+    const Plan p = plan_of(a);
+    const int group = a.n_heads / a.pool.n_kv;
+    const long long blocks = (long long)a.bt.nseq * a.pool.n_kv * p.tiles * p.splits;
+    if (blocks > 0x7fffffffLL / 256) return note_error(hipErrorInvalidConfiguration);
+    const dim3 grid((unsigned)blocks);
+    auto go = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, dim3(DC_WAVES * 64), 0, stream, a, group, p.tiles, p.splits, p.per); };
+    if (p.nt == 1) go(paged_decode_kernel<T, KVF, HD, 1>);
+    else go(paged_decode_kernel<T, KVF, HD, 2>);
+    if (p.splits > 1) {
+        const long long n = (long long)a.bt.max_rows * a.n_heads * (HD / 4);
+        hipLaunchKernelGGL((paged_merge_kernel<T, HD>), dim3((unsigned)((n + 255) / 256), a.bt.nseq), dim3(256), 0, stream, a, p.splits);
+    }
     return note_error(hipGetLastError());
+}
+
+template <typename T, int KVF>
+int launch_kv(const PagedAttnArgs& a, hipStream_t stream) {
+    return a.pool.hd == 128 ? launch_hd<T, KVF, 128>(a, stream) : launch_hd<T, KVF, 64>(a, stream);
 }
 
 }  // namespace
 
-long long paged_attention_workspace(const PagedAttnArgs&) { return 0; }
+long long paged_attention_workspace(const PagedAttnArgs& a) {
+    const Plan p = plan_of(a);
+    return p.splits > 1 ? (long long)p.splits * a.bt.rows * a.n_heads * (a.pool.hd + 2) * 4 : 0;
+}
 
 int launch_paged_attention(const PagedAttnArgs& a, hipStream_t stream) {
     if (a.act == ACT_F32)
-        return a.pool.fmt == KV_INT8 ? launch_hd<float, int8_t, true>(a, stream)
-                                     : launch_hd<float, _Float16, false>(a, stream);
+        return a.pool.fmt == KV_INT8 ? launch_kv<float, KV_INT8>(a, stream) : launch_kv<float, KV_F16>(a, stream);
     if (a.act == ACT_F16)
-        return a.pool.fmt == KV_INT8 ? launch_hd<_Float16, int8_t, true>(a, stream)
-                                     : launch_hd<_Float16, _Float16, false>(a, stream);
-    return launch_hd<__bf16, __bf16, false>(a, stream);
+        return a.pool.fmt == KV_INT8 ? launch_kv<_Float16, KV_INT8>(a, stream) : launch_kv<_Float16, KV_F16>(a, stream);
+    return launch_kv<__bf16, KV_BF16>(a, stream);
 }
 
 }  // namespace aarh
