@@ -467,9 +467,344 @@ __global__ __launch_bounds__(256) void paged_merge_kernel(PagedAttnArgs a, int s
 }
 
 // ---------------------------------------------------------------------------
+// Many rows: tiles of 128 rows share each block through LDS
+//
+// Four waves of 32 columns each (32 x 32 matrix instructions: an operand read from LDS serves 32 queries). 64 tokens a
+// step, two steps' pages in LDS: the next step's loads go straight to LDS while this one is computed.
+// V^T pieces are placed so that the lanes of a read (consecutive dimensions, one token octet) fall on
+// different banks: piece (dimension d, octet q) of a 16-dimension KiB sits at 4 d + (q ^ f(d)).
+// ---------------------------------------------------------------------------
+typedef float float16_t __attribute__((ext_vector_type(16)));
+
+template <int KVF>
+__device__ __forceinline__ float16_t mfma32(typename Mat<KVF>::frag a, typename Mat<KVF>::frag b, float16_t c) {
+    if constexpr (KVF == KV_BF16) return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
+    else return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
+}
+__device__ __forceinline__ float half_max(float x) {
+    auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
+}
+__device__ __forceinline__ float half_sum(float x) {
+    auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return __uint_as_float(b[0]) + __uint_as_float(b[1]);
+}
+
+constexpr int PF_WAVES = 4, PF_ROWS = 32 * PF_WAVES;
+
+template <typename T, int KVF, int HD>
+__global__ __launch_bounds__(PF_WAVES * 64, 2) void paged_prompt_kernel(PagedAttnArgs a, int group, int tiles, int splits, int per) {
+    typedef typename Mat<KVF>::frag frag;
+    typedef typename Mat<KVF>::elem elem;
+    constexpr bool I8 = KVF == KV_INT8, F32 = std::is_same<T, float>::value;
+    constexpr int KS = HD / 16;  // k-steps of K Q^T: (64-dimension part, half of 16, pair of lane groups)
+    constexpr int DT = HD / 32;  // 32-dimension tiles of O^T
+    constexpr int BLK = PAGE_BLK * HD * (I8 ? 1 : 2);
+    constexpr int KIB = BLK / 1024;  // wave loads of a block of K (or V)
+    extern __shared__ char pf_lds[];  // [2 stages][K: 2 blocks | V: 2 blocks]
+    const int tid = threadIdx.x, lane = tid & 63, wid = __builtin_amdgcn_readfirstlane(tid >> 6), hk = lane >> 5, m = lane & 31;
+    int id = blockIdx.x;
+    const int pairs = a.bt.nseq * a.pool.n_kv;
+    const int pair = id % pairs;
+    id /= pairs;
+    const int tile = tiles - 1 - id % tiles, split = id / tiles;  // the longest rows first
+    TileInfo t;
+    if (!tile_info(a, pair / a.pool.n_kv, pair % a.pool.n_kv, tile, PF_ROWS, group, &t)) return;
+    const int k0 = split * per, k1 = min(k0 + per, t.n);
+    const int rows = t.s.rows * group, pos0 = t.s.kv_len - t.s.rows;
+
+    // this lane's query
+    const int r = t.r0 + wid * 32 + m, rr = min(r, rows - 1), tok = rr / group;
+    const int h = head_of(a, t.kvh, rr - tok * group, group);
+    const int pos = pos0 + tok;
+    const float slope = a.slopes ? a.slopes[h] * PA_LOG2E : 0.f;
+    const int w_lo = pos0 + min(t.r0 + wid * 32, rows - 1) / group, w_hi = pos0 + min(t.r0 + wid * 32 + 31, rows - 1) / group;
+    const bool idle = t.r0 + wid * 32 >= rows;  // a wave without rows
+    frag qh[KS], ql[F32 ? KS : 1];
+    float qs = a.scale;
+    {
+        const T* q = (const T*)a.q + (long long)(t.s.row0 + tok) * a.q_ld + (long long)h * HD + 16 * hk;
+        auto dim = [](int ks) { return 64 * (ks >> 2) + 32 * (ks & 1) + 8 * ((ks >> 1) & 1); };
+        if constexpr (F32) {
+            float x[KS][8], top = 0.f;
+#pragma unroll
+            for (int ks = 0; ks < KS; ks++) {
+                const float4_t u = *(const float4_t*)(q + dim(ks)), v = *(const float4_t*)(q + dim(ks) + 4);
+#pragma unroll
+                for (int j = 0; j < 4; j++) {
+                    x[ks][j] = u[j];
+                    x[ks][4 + j] = v[j];
+                }
+#pragma unroll
+                for (int j = 0; j < 8; j++) top = fmaxf(top, fabsf(x[ks][j]));
+            }
+            const int e = max(__builtin_amdgcn_frexp_expf(half_max(top)), -120);
+            const float inv = ldexpf(1.f, -e);
+            qs = ldexpf(a.scale, e);
+#pragma unroll
+            for (int ks = 0; ks < KS; ks++)
+#pragma unroll
+                for (int j = 0; j < 8; j++) {
+                    const float v = x[ks][j] * inv;
+                    qh[ks][j] = (_Float16)v;
+                    ql[ks][j] = (_Float16)(v - (float)qh[ks][j]);
+                }
+        } else {
+#pragma unroll
+            for (int ks = 0; ks < KS; ks++) {
+                if constexpr (std::is_same<T, elem>::value) qh[ks] = *(const frag*)(q + dim(ks));
+            }
+        }
+    }
+
+    const int32_t* table = a.bt.tables + t.b * a.bt.table_ld;
+    const int shift = a.pool.page_shift - 5;
+    const bool plain = a.softcap == 0.f && a.slopes == nullptr;
+    // lane's places in LDS: K token row (bits 2 and 3 of its number change places: see paged_rule.hpp), V piece
+    const int k_lane = ((m >> 3) & 1) * (BLK / 2) + hk * 256 + (8 * (m >> 4) + 4 * ((m >> 2) & 1) + (m & 3)) * 16;
+    auto swz = [](int d) { return ((d >> 1) & 3) ^ ((d >> 3) & 1); };
+    const int v_lane = I8 ? hk * 256 + (m & 15) * 16 + (m >> 4) * 8 : (m >> 4) * 1024 + (m & 15) * 64 + ((hk ^ swz(m & 15)) << 4);
+    const int v_src = I8 ? lane * 16 : ((lane & ~3) + ((lane & 3) ^ swz(lane >> 2))) * 16;  // global piece for LDS place `lane`
+
+    struct Step {
+        int t0[2], page[2];
+        size_t off[2];  // token offset of the blocks in the scale arrays; x HD elements in K and V
+    };
+    auto step_at = [&](int k) __attribute__((always_inline)) {
+        Step s;
+#pragma unroll
+        for (int j = 0; j < 2; j++) {
+            const int blk = tile_block(t, min(k + j, k1 - 1));
+            s.t0[j] = blk * PAGE_BLK;
+            int p = __builtin_amdgcn_readfirstlane(table[blk >> shift]);
+            if (p < 0 || p >= a.pool.n_pages) p = -1;
+            s.page[j] = p;
+            s.off[j] = ((((size_t)max(p, 0) * a.pool.n_kv + t.kvh) << shift) + (blk & ((1 << shift) - 1))) * PAGE_BLK;
+        }
+        return s;
+    };
+    auto stage = [&](const Step& s, int buf) __attribute__((always_inline)) {
+        char* base = pf_lds + buf * (4 * BLK);
+#pragma unroll
+        for (int j = 0; j < 2; j++) {
+            const __amdgpu_buffer_rsrc_t kr = coh_rsrc((const char*)a.pool.k + s.off[j] * (BLK / PAGE_BLK));
+            const __amdgpu_buffer_rsrc_t vr = coh_rsrc((const char*)a.pool.v + s.off[j] * (BLK / PAGE_BLK));
+#pragma unroll
+            for (int i = 0; i < KIB / PF_WAVES + (KIB % PF_WAVES != 0); i++) {
+                const int p = i * PF_WAVES + wid;
+                if (KIB % PF_WAVES && p >= KIB) break;
+                lds_dma16(kr, base + j * BLK + p * 1024, lane * 16, p * 1024);
+                lds_dma16(vr, base + (2 + j) * BLK + p * 1024, v_src, p * 1024);
+            }
+        }
+    };
+
+    float mx_run = -INFINITY, l = 0.f;
+    float16_t o[DT];
+#pragma unroll
+    for (int d = 0; d < DT; d++)
+#pragma unroll
+        for (int i = 0; i < 16; i++) o[d][i] = 0.f;
+    bool bad = false;
+    Step cur{}, nxt{};
+    if (k0 < k1) {
+        nxt = step_at(k0);
+        stage(nxt, 0);
+    }
+    for (int k = k0, buf = 0; k < k1; k += 2, buf ^= 1) {
+        cur = nxt;
+        wait_vmcnt<0>();
+        __syncthreads();  // this step has landed for every wave, and the other stage is free
+        if (k + 2 < k1) {
+            nxt = step_at(k + 2);
+            stage(nxt, buf ^ 1);
+        }
+        const bool two = k + 1 < k1;
+        bad |= cur.page[0] < 0 || (two && cur.page[1] < 0);
+        // blocks that no row of this wave sees
+        auto unseen = [&](int t0) { return t0 > w_hi && t0 >= t.pre; };
+        const int wlow = a.window ? max(0, w_lo - a.window + 1) : 0;
+        auto before = [&](int t0) { return t0 + PAGE_BLK <= wlow && t0 >= t.pre; };
+        const bool skip0 = cur.page[0] < 0 || unseen(cur.t0[0]) || before(cur.t0[0]);
+        const bool skip1 = !two || cur.page[1] < 0 || unseen(cur.t0[1]) || before(cur.t0[1]);
+        if (idle || (skip0 && skip1)) continue;
+        const char* kb = pf_lds + buf * (4 * BLK) + k_lane;
+        const char* vb = pf_lds + buf * (4 * BLK) + 2 * BLK;
+        float16_t s[2];
+#pragma unroll
+        for (int j = 0; j < 2; j++) {
+#pragma unroll
+            for (int i = 0; i < 16; i++) s[j][i] = 0.f;
+            if constexpr (I8) {
+#pragma unroll
+                for (int c = 0; c < KS / 4; c++)
+#pragma unroll
+                    for (int g = 0; g < 2; g++) {
+                        const u32x4_t w = *(const u32x4_t*)(kb + j * BLK + c * 1024 + g * 512);
+#pragma unroll
+                        for (int half = 0; half < 2; half++) {
+                            const half8_t ka = half ? i8_to_half8(w[2], w[3]) : i8_to_half8(w[0], w[1]);
+                            const int ks = c * 4 + half * 2 + g;
+                            s[j] = mfma32<KVF>(ka, qh[ks], s[j]);
+                            if constexpr (F32) s[j] = mfma32<KVF>(ka, ql[ks], s[j]);
+                        }
+                    }
+            } else {
+#pragma unroll
+                for (int ks = 0; ks < KS; ks++) {
+                    const frag ka = *(const frag*)(kb + j * BLK + (ks >> 1) * 1024 + (ks & 1) * 512);
+                    s[j] = mfma32<KVF>(ka, qh[ks], s[j]);
+                    if constexpr (F32) s[j] = mfma32<KVF>(ka, ql[ks], s[j]);
+                }
+            }
+        }
+        auto whole_at = [&](int t0) {
+            return t0 + PAGE_BLK - 1 <= w_lo && (a.window == 0 || t0 > w_hi - a.window || t0 + PAGE_BLK <= t.pre);
+        };
+        const bool whole = !skip0 && !skip1 && whole_at(cur.t0[0]) && whole_at(cur.t0[1]);
+        float vsc[2][I8 ? 16 : 1];
+        float vexp = 0.f;
+        if constexpr (I8) {
+            float top = 0.f;
+#pragma unroll
+            for (int j = 0; j < 2; j++)
+#pragma unroll
+                for (int g = 0; g < 2; g++) {
+                    const half8_t ksc = *(const half8_t*)(a.pool.ks + cur.off[j] + 16 * g + 8 * hk);
+                    const half8_t vs = *(const half8_t*)(a.pool.vs + cur.off[j] + 16 * g + 8 * hk);
+#pragma unroll
+                    for (int i = 0; i < 8; i++) {
+                        s[j][8 * g + i] *= (float)ksc[i];
+                        const float v = (float)vs[i];
+                        vsc[j][8 * g + i] = v;
+                        top = fmaxf(top, cur.t0[j] + 16 * g + 8 * hk + i < t.s.kv_len ? v : 0.f);
+                    }
+                }
+            top = half_max(top);
+            vexp = top > 0x1p-20f ? (float)__builtin_amdgcn_frexp_expf(top) : -20.f;
+        }
+        if (plain) {
+            const float c = qs * PA_LOG2E;
+#pragma unroll
+            for (int j = 0; j < 2; j++)
+#pragma unroll
+                for (int i = 0; i < 16; i++) s[j][i] *= c;
+        } else {
+#pragma unroll
+            for (int j = 0; j < 2; j++)
+#pragma unroll
+                for (int i = 0; i < 16; i++) {
+                    float x = s[j][i] * qs;
+                    if (a.softcap > 0.f) x = a.softcap * tanh_f32(x / a.softcap);
+                    s[j][i] = x * PA_LOG2E + slope * (float)(cur.t0[j] + 16 * (i >> 3) + 8 * hk + (i & 7) - pos);
+                }
+        }
+        if (!whole) {
+#pragma unroll
+            for (int j = 0; j < 2; j++)
+#pragma unroll
+                for (int i = 0; i < 16; i++) {
+                    const int tk = cur.t0[j] + 16 * (i >> 3) + 8 * hk + (i & 7);
+                    const bool seen = !(j ? skip1 : skip0) && ((tk <= pos && (a.window == 0 || pos - tk < a.window)) || tk < t.pre);
+                    s[j][i] = seen ? s[j][i] : -INFINITY;
+                }
+        }
+        float mx = s[0][0];
+#pragma unroll
+        for (int i = 1; i < 16; i++) mx = fmaxf(mx, s[0][i]);
+#pragma unroll
+        for (int i = 0; i < 16; i++) mx = fmaxf(mx, s[1][i]);
+        mx = half_max(mx);
+        if constexpr (I8) mx += vexp;
+        const float mn = fmaxf(mx_run, mx);
+        if (__any(mn > mx_run)) {
+            const float alpha = mn == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(mx_run - mn);
+            l *= alpha;
+#pragma unroll
+            for (int d = 0; d < DT; d++) o[d] *= alpha;
+            mx_run = mn;
+        }
+        const float ref = (mn == -INFINITY ? 0.f : mn) - Mat<KVF>::P_BITS;
+        frag ph[2][2], pl[F32 ? 2 : 1][2];
+#pragma unroll
+        for (int j = 0; j < 2; j++)
+#pragma unroll
+            for (int i = 0; i < 16; i++) {
+                float p = __builtin_amdgcn_exp2f(s[j][i] - ref);
+                l += p;
+                if constexpr (I8) p = s[j][i] == -INFINITY ? 0.f : p * vsc[j][i];
+                ph[j][i >> 3][i & 7] = (elem)p;
+                if constexpr (F32) pl[j][i >> 3][i & 7] = (elem)(p - (float)ph[j][i >> 3][i & 7]);
+            }
+#pragma unroll
+        for (int j = 0; j < 2; j++) {
+#pragma unroll
+            for (int g = 0; g < 2; g++) {
+                u32x4_t keep;
+                if constexpr (!I8) {
+                    // tokens that no row of this wave sees may hold anything, also NaN
+                    if (!whole) {
+#pragma unroll
+                        for (int i = 0; i < 4; i++) {
+                            uint32_t w = 0;
+#pragma unroll
+                            for (int e = 0; e < 2; e++) {
+                                const int tk = cur.t0[j] + 16 * g + 8 * hk + 2 * i + e;
+                                const bool any = !(j ? skip1 : skip0) && ((tk <= w_hi && tk >= wlow) || tk < t.pre);
+                                w |= any ? 0xFFFFu << (16 * e) : 0u;
+                            }
+                            keep[i] = w;
+                        }
+                    }
+                }
+#pragma unroll
+                for (int d = 0; d < DT; d++) {
+                    frag va;
+                    if constexpr (I8) {
+                        const uint2 w = *(const uint2*)(vb + j * BLK + v_lane + d * 1024 + g * 512);
+                        va = i8_to_half8(w.x, w.y);
+                    } else {
+                        u32x4_t w = *(const u32x4_t*)(vb + j * BLK + (v_lane ^ (g * 32)) + d * 2048);
+                        if (!whole) w &= keep;
+                        va = __builtin_bit_cast(frag, w);
+                    }
+                    o[d] = mfma32<KVF>(va, ph[j][g], o[d]);
+                    if constexpr (F32) o[d] = mfma32<KVF>(va, pl[j][g], o[d]);
+                }
+            }
+        }
+    }
+    if (bad && a.bt.status && tid == 0) atomicOr(&a.bt.status[t.b], PAGE_SEQ_BAD_PAGE);
+    l = half_sum(l);
+    if (r >= rows) return;
+    const long long row = t.s.row0 + tok;
+    if (splits > 1) {
+        const long long slot = row * a.n_heads + h;
+        float* po = part_o(a, split, slot) + 4 * hk;
+#pragma unroll
+        for (int d = 0; d < DT; d++)
+#pragma unroll
+            for (int g = 0; g < 4; g++)
+                *(float4_t*)(po + 32 * d + 8 * g) = float4_t{o[d][4 * g], o[d][4 * g + 1], o[d][4 * g + 2], o[d][4 * g + 3]};
+        if (hk == 0) *part_ml(a, splits, split, slot) = float2_t{mx_run, l};
+        return;
+    }
+    const float inv = l > 0.f ? 1.f / l : 0.f;
+    T* out = (T*)a.out + row * a.out_ld + (long long)h * HD + 4 * hk;
+    typedef T out4 __attribute__((ext_vector_type(4)));
+#pragma unroll
+    for (int d = 0; d < DT; d++)
+#pragma unroll
+        for (int g = 0; g < 4; g++)
+            *(out4*)(out + 32 * d + 8 * g) = out4{(T)(o[d][4 * g] * inv), (T)(o[d][4 * g + 1] * inv), (T)(o[d][4 * g + 2] * inv),
+                                                  (T)(o[d][4 * g + 3] * inv)};
+}
+
+// ---------------------------------------------------------------------------
 // launch plan
 // ---------------------------------------------------------------------------
 struct Plan {
+    bool prompt;
     int nt, tiles, splits, per;  // 16-row column tiles of a workgroup, tiles of a (sequence, kv head), splits, blocks each
 };
 
@@ -477,18 +812,21 @@ Plan plan_of(const PagedAttnArgs& a) {
     const int group = a.n_heads / a.pool.n_kv;
     const long long rows = (long long)a.bt.max_rows * group;
     Plan p{};
+    p.prompt = rows > 32;
     p.nt = rows <= 16 ? 1 : 2;
-    p.tiles = (int)((rows + 16 * p.nt - 1) / (16 * p.nt));
+    const int tile_rows = p.prompt ? PF_ROWS : 16 * p.nt;
+    p.tiles = (int)((rows + tile_rows - 1) / tile_rows);
     // blocks that a tile can visit
     const int all = (a.bt.max_kv + 31) / 32;
-    const int span = (16 * p.nt + group - 1) / group + 1;
-    const int n = a.window && !a.prefix ? std::min<long long>(all, ((long long)a.window + span) / 32 + 2) : all;
-    // two workgroups per compute unit; a wave gets at least two blocks
+    const int span = (tile_rows + group - 1) / group + 1;
+    const int n = a.window && !a.prefix ? (int)std::min<long long>(all, ((long long)a.window + span) / 32 + 2) : all;
+    // two workgroups per compute unit; a wave (or a workgroup that shares its blocks) gets at least two blocks or steps
     const long long base = (long long)a.bt.nseq * a.pool.n_kv * p.tiles;
     const int want = (int)std::max<long long>(1, (512 + base - 1) / base);
-    p.splits = std::max(1, std::min(want, n / (2 * DC_WAVES)));
+    const int unit = p.prompt ? 2 : DC_WAVES;
+    p.splits = std::max(1, std::min(want, n / (2 * unit)));
     p.per = (n + p.splits - 1) / p.splits;
-    p.per = (p.per + DC_WAVES - 1) / DC_WAVES * DC_WAVES;
+    p.per = (p.per + unit - 1) / unit * unit;
     p.splits = std::max(1, (n + p.per - 1) / p.per);
     return p;
 }
@@ -500,9 +838,12 @@ int launch_hd(const PagedAttnArgs& a, hipStream_t stream) {
     const long long blocks = (long long)a.bt.nseq * a.pool.n_kv * p.tiles * p.splits;
     if (blocks > 0x7fffffffLL / 256) return note_error(hipErrorInvalidConfiguration);
     const dim3 grid((unsigned)blocks);
-    auto go = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, dim3(DC_WAVES * 64), 0, stream, a, group, p.tiles, p.splits, p.per); };
-    if (p.nt == 1) go(paged_decode_kernel<T, KVF, HD, 1>);
-    else go(paged_decode_kernel<T, KVF, HD, 2>);
+    auto go = [&](auto kernel, unsigned lds) {
+        hipLaunchKernelGGL(kernel, grid, dim3(256), lds, stream, a, group, p.tiles, p.splits, p.per);
+    };
+    if (p.prompt) go(paged_prompt_kernel<T, KVF, HD>, 8 * PAGE_BLK * HD * (KVF == KV_INT8 ? 1 : 2));
+    else if (p.nt == 1) go(paged_decode_kernel<T, KVF, HD, 1>, 0);
+    else go(paged_decode_kernel<T, KVF, HD, 2>, 0);
     if (p.splits > 1) {
         const long long n = (long long)a.bt.max_rows * a.n_heads * (HD / 4);
         hipLaunchKernelGGL((paged_merge_kernel<T, HD>), dim3((unsigned)((n + 255) / 256), a.bt.nseq), dim3(256), 0, stream, a, p.splits);
