@@ -30,9 +30,11 @@ template <int KVF>
 struct Mat {
     typedef typename std::conditional<KVF == KV_BF16, bfrag_t, half8_t>::type frag;
     typedef typename std::conditional<KVF == KV_BF16, __bf16, _Float16>::type elem;
-    // fp16 weights are scaled by 2^14 (a power of two in the exponent's argument, cancelled by the sum): the
-    // smallest steps of fp16 are then 2^-38 of the largest weight
-    static constexpr float P_BITS = KVF == KV_BF16 ? 0.f : 14.f;
+    // The running reference of a column's exponents follows its maximum only when that is past it by
+    // P_LAG (in powers of two), so most blocks leave O as it is.  fp16 weights are scaled by 2^P_BITS (cancelled by the sum):
+    // the largest lies between 2^11 and 2^15, and the smallest steps of fp16 are 2^-35 of it.
+    static constexpr float P_LAG = 4.f;
+    static constexpr float P_BITS = KVF == KV_BF16 ? 0.f : 11.f;
 };
 
 template <int KVF>
@@ -71,13 +73,15 @@ __device__ __forceinline__ float row16_sum(float x) {
     return __uint_as_float(b[0]) + __uint_as_float(b[1]);
 }
 
-// tanh to a few units: a series where the quotient would cancel
+// tanh(x) = 1 - 2 / (exp(2 x) + 1).  Near zero that is off by 2^-23 absolutely, which a score of 16-bit
+// operands does not notice; PRECISE takes the series there.
+template <bool PRECISE>
 __device__ __forceinline__ float tanh_f32(float x) {
-    const float y = fabsf(x), y2 = y * y;
-    const float series = y * (1.f + y2 * (-0.33333333333f + y2 * (0.13333333333f + y2 * (-0.053968253968f + y2 * (0.021869488536f - y2 * 0.0088632355299f)))));
-    const float e = __builtin_amdgcn_exp2f(y * (2.f * PA_LOG2E));
-    const float big = 1.f - 2.f / (e + 1.f);
-    return copysignf(y < 0.3f ? series : big, x);
+    const float big = 1.f - 2.f * __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(x * (2.f * PA_LOG2E)) + 1.f);
+    if constexpr (!PRECISE) return big;
+    const float y2 = x * x;
+    const float series = x * (1.f + y2 * (-0.33333333333f + y2 * (0.13333333333f + y2 * (-0.053968253968f + y2 * (0.021869488536f - y2 * 0.0088632355299f)))));
+    return fabsf(x) < 0.3f ? series : big;
 }
 
 // What a tile of query rows needs to know of its sequence.
@@ -167,7 +171,7 @@ __global__ __launch_bounds__(DC_WAVES * 64, 2) void paged_decode_kernel(PagedAtt
         pos[nt] = r < rows ? pos0 + tok : -1;  // -1: a column of no row, sees at most prefix keys
         slope[nt] = a.slopes ? a.slopes[h] * PA_LOG2E : 0.f;
         const T* q = (const T*)a.q + (long long)(t.s.row0 + tok) * a.q_ld + (long long)h * HD + 16 * lg;
-        qs[nt] = a.scale;
+        qs[nt] = fabsf(a.scale);
         if constexpr (F32) {
             float x[KS][8], top = 0.f;
 #pragma unroll
@@ -185,7 +189,7 @@ __global__ __launch_bounds__(DC_WAVES * 64, 2) void paged_decode_kernel(PagedAtt
             // a power of two brings the row's largest value to [1/2, 1) (fp16's range); the scale takes it back
             const int e = __builtin_amdgcn_frexp_expf(row16_max(top));
             const float inv = ldexpf(1.f, -max(e, -120));
-            qs[nt] = ldexpf(a.scale, max(e, -120));
+            qs[nt] = ldexpf(qs[nt], max(e, -120));
 #pragma unroll
             for (int ks = 0; ks < KS; ks++)
 #pragma unroll
@@ -200,6 +204,14 @@ __global__ __launch_bounds__(DC_WAVES * 64, 2) void paged_decode_kernel(PagedAtt
                 if constexpr (std::is_same<T, elem>::value) qh[nt][ks] = *(const frag*)(q + 64 * (ks >> 1) + 8 * (ks & 1));
             }
         }
+        if (a.scale < 0.f) {  // a negative scale's sign goes to the query, so that the largest product is the largest score
+#pragma unroll
+            for (int ks = 0; ks < KS; ks++) {
+                qh[nt][ks] = -qh[nt][ks];
+                if constexpr (F32) ql[nt][ks] = -ql[nt][ks];
+            }
+        }
+        qs[nt] = fmaxf(qs[nt], 1e-30f);  // -inf of a masked key stays what it is
     }
 
     float m[NT], l[NT];
@@ -215,6 +227,7 @@ __global__ __launch_bounds__(DC_WAVES * 64, 2) void paged_decode_kernel(PagedAtt
     const int32_t* table = a.bt.tables + t.b * a.bt.table_ld;
     const int shift = a.pool.page_shift - 5;  // blocks of a page
     const bool plain = a.softcap == 0.f && a.slopes == nullptr;
+    const float inv_cap = a.softcap > 0.f ? 1.f / a.softcap : 0.f;
     u32x4_t kr[KL], vr[KL], ksc, vsc;
     // this wave's blocks: k0 + wid, k0 + wid + DC_WAVES, ..
     auto page_at = [&](int k) __attribute__((always_inline)) {
@@ -309,17 +322,15 @@ __global__ __launch_bounds__(DC_WAVES * 64, 2) void paged_decode_kernel(PagedAtt
                 x[i] = s[nt][i >> 2][i & 3];
                 if constexpr (I8) x[i] *= sc_at(ksc_now, i);
             }
-            if (plain) {
-                const float c = qs[nt] * PA_LOG2E;
-#pragma unroll
-                for (int i = 0; i < 8; i++) x[i] *= c;
-            } else {
+            float c = qs[nt] * PA_LOG2E;
+            if (!plain) {
 #pragma unroll
                 for (int i = 0; i < 8; i++) {
                     x[i] *= qs[nt];
-                    if (a.softcap > 0.f) x[i] = a.softcap * tanh_f32(x[i] / a.softcap);
+                    if (a.softcap > 0.f) x[i] = a.softcap * tanh_f32<F32>(x[i] * inv_cap);
                     x[i] = x[i] * PA_LOG2E + slope[nt] * (float)(t0 + 8 * lg + i - pos[nt]);
                 }
+                c = 1.f;
             }
             if (!whole) {
 #pragma unroll
@@ -332,24 +343,23 @@ __global__ __launch_bounds__(DC_WAVES * 64, 2) void paged_decode_kernel(PagedAtt
             float mx = x[0];
 #pragma unroll
             for (int i = 1; i < 8; i++) mx = fmaxf(mx, x[i]);
-            mx = row16_max(mx);
+            mx = row16_max(mx) * c;
             if constexpr (I8) mx += vexp;
-            const float mn = fmaxf(m[nt], mx);
-            // rescale only when some column's maximum moved
-            if (__any(mn > m[nt])) {
+            if (__any(mx > m[nt] + Mat<KVF>::P_LAG)) {
+                const float mn = fmaxf(m[nt], mx);
                 const float alpha = mn == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m[nt] - mn);
                 l[nt] *= alpha;
 #pragma unroll
                 for (int d = 0; d < DT; d++) o[nt][d] *= alpha;
                 m[nt] = mn;
             }
-            const float ref = (mn == -INFINITY ? 0.f : mn) - Mat<KVF>::P_BITS;
+            const float ref = (m[nt] == -INFINITY ? 0.f : m[nt]) - Mat<KVF>::P_BITS;
             float p[8];
 #pragma unroll
             for (int i = 0; i < 8; i++) {
-                p[i] = __builtin_amdgcn_exp2f(x[i] - ref);
+                p[i] = __builtin_amdgcn_exp2f(fmaf(x[i], c, -ref));
                 l[nt] += p[i];
-                if constexpr (I8) p[i] = x[i] == -INFINITY ? 0.f : p[i] * sc_at(vsc, i);
+                if constexpr (I8) p[i] = p[i] == 0.f ? 0.f : p[i] * sc_at(vsc, i);  // a token that is not there may have any scale
             }
 #pragma unroll
             for (int i = 0; i < 8; i++) {
@@ -490,9 +500,42 @@ __device__ __forceinline__ float half_sum(float x) {
     return __uint_as_float(b[0]) + __uint_as_float(b[1]);
 }
 
+// N consecutive KiB (global and LDS) in one go, as lds_dma16 (the instruction offset moves both addresses).
+template <int N>
+__device__ __forceinline__ void lds_dma_kib(__amdgpu_buffer_rsrc_t r, const void* lds_dst, int voff, int soff) {
+    static_assert(N == 2 || N == 4, "two or four KiB");
+    const unsigned base = __builtin_amdgcn_readfirstlane((unsigned)(uintptr_t)lds_dst);
+    int saved;
+    if constexpr (N == 2)
+        asm volatile(
+            "s_mov_b32 %0, m0\n\t"
+            "s_mov_b32 m0, %1\n\t"
+            "s_nop 0\n\t"
+            "buffer_load_dwordx4 %2, %3, %4 offen lds\n\t"
+            "buffer_load_dwordx4 %2, %3, %4 offen offset:1024 lds\n\t"
+            "s_mov_b32 m0, %0"
+            : "=&s"(saved)
+            : "s"(base), "v"(voff), "s"(r), "s"(soff)
+            : "memory");
+    else
+        asm volatile(
+            "s_mov_b32 %0, m0\n\t"
+            "s_mov_b32 m0, %1\n\t"
+            "s_nop 0\n\t"
+            "buffer_load_dwordx4 %2, %3, %4 offen lds\n\t"
+            "buffer_load_dwordx4 %2, %3, %4 offen offset:1024 lds\n\t"
+            "buffer_load_dwordx4 %2, %3, %4 offen offset:2048 lds\n\t"
+            "buffer_load_dwordx4 %2, %3, %4 offen offset:3072 lds\n\t"
+            "s_mov_b32 m0, %0"
+            : "=&s"(saved)
+            : "s"(base), "v"(voff), "s"(r), "s"(soff)
+            : "memory");
+}
+
 constexpr int PF_WAVES = 4, PF_ROWS = 32 * PF_WAVES;
 
-template <typename T, int KVF, int HD>
+// MODE 0: scores as they are, 1: capped, 2: a slope per head (capped or not)
+template <typename T, int KVF, int HD, int MODE>
 __global__ __launch_bounds__(PF_WAVES * 64, 2) void paged_prompt_kernel(PagedAttnArgs a, int group, int tiles, int splits, int per) {
     typedef typename Mat<KVF>::frag frag;
     typedef typename Mat<KVF>::elem elem;
@@ -517,11 +560,11 @@ __global__ __launch_bounds__(PF_WAVES * 64, 2) void paged_prompt_kernel(PagedAtt
     const int r = t.r0 + wid * 32 + m, rr = min(r, rows - 1), tok = rr / group;
     const int h = head_of(a, t.kvh, rr - tok * group, group);
     const int pos = pos0 + tok;
-    const float slope = a.slopes ? a.slopes[h] * PA_LOG2E : 0.f;
+    const float slope = MODE == 2 ? a.slopes[h] * PA_LOG2E : 0.f;
     const int w_lo = pos0 + min(t.r0 + wid * 32, rows - 1) / group, w_hi = pos0 + min(t.r0 + wid * 32 + 31, rows - 1) / group;
     const bool idle = t.r0 + wid * 32 >= rows;  // a wave without rows
     frag qh[KS], ql[F32 ? KS : 1];
-    float qs = a.scale;
+    float qs = fabsf(a.scale);
     {
         const T* q = (const T*)a.q + (long long)(t.s.row0 + tok) * a.q_ld + (long long)h * HD + 16 * hk;
         auto dim = [](int ks) { return 64 * (ks >> 2) + 32 * (ks & 1) + 8 * ((ks >> 1) & 1); };
@@ -540,7 +583,7 @@ __global__ __launch_bounds__(PF_WAVES * 64, 2) void paged_prompt_kernel(PagedAtt
             }
             const int e = max(__builtin_amdgcn_frexp_expf(half_max(top)), -120);
             const float inv = ldexpf(1.f, -e);
-            qs = ldexpf(a.scale, e);
+            qs = ldexpf(qs, e);
 #pragma unroll
             for (int ks = 0; ks < KS; ks++)
 #pragma unroll
@@ -555,48 +598,62 @@ __global__ __launch_bounds__(PF_WAVES * 64, 2) void paged_prompt_kernel(PagedAtt
                 if constexpr (std::is_same<T, elem>::value) qh[ks] = *(const frag*)(q + dim(ks));
             }
         }
+        if (a.scale < 0.f) {  // a negative scale's sign goes to the query, so that the largest product is the largest score
+#pragma unroll
+            for (int ks = 0; ks < KS; ks++) {
+                qh[ks] = -qh[ks];
+                if constexpr (F32) ql[ks] = -ql[ks];
+            }
+        }
+        qs = fmaxf(qs, 1e-30f);  // -inf of a masked key stays what it is
     }
 
     const int32_t* table = a.bt.tables + t.b * a.bt.table_ld;
     const int shift = a.pool.page_shift - 5;
-    const bool plain = a.softcap == 0.f && a.slopes == nullptr;
+    const bool capped = a.softcap > 0.f;
+    const float inv_cap = capped ? 1.f / a.softcap : 0.f, cap2 = a.softcap * PA_LOG2E;
     // lane's places in LDS: K token row (bits 2 and 3 of its number change places: see paged_rule.hpp), V piece
     const int k_lane = ((m >> 3) & 1) * (BLK / 2) + hk * 256 + (8 * (m >> 4) + 4 * ((m >> 2) & 1) + (m & 3)) * 16;
     auto swz = [](int d) { return ((d >> 1) & 3) ^ ((d >> 3) & 1); };
     const int v_lane = I8 ? hk * 256 + (m & 15) * 16 + (m >> 4) * 8 : (m >> 4) * 1024 + (m & 15) * 64 + ((hk ^ swz(m & 15)) << 4);
     const int v_src = I8 ? lane * 16 : ((lane & ~3) + ((lane & 3) ^ swz(lane >> 2))) * 16;  // global piece for LDS place `lane`
 
+    // Blocks of a step, two: their numbers in the sequence and pages (wave-uniform).  A step's pages are read
+    // a step before its loads are issued, and these a step before the data is needed.
     struct Step {
-        int t0[2], page[2];
-        size_t off[2];  // token offset of the blocks in the scale arrays; x HD elements in K and V
+        int blk[2], page[2];
     };
-    auto step_at = [&](int k) __attribute__((always_inline)) {
+    auto look_up = [&](int k) __attribute__((always_inline)) {
         Step s;
 #pragma unroll
         for (int j = 0; j < 2; j++) {
-            const int blk = tile_block(t, min(k + j, k1 - 1));
-            s.t0[j] = blk * PAGE_BLK;
-            int p = __builtin_amdgcn_readfirstlane(table[blk >> shift]);
-            if (p < 0 || p >= a.pool.n_pages) p = -1;
-            s.page[j] = p;
-            s.off[j] = ((((size_t)max(p, 0) * a.pool.n_kv + t.kvh) << shift) + (blk & ((1 << shift) - 1))) * PAGE_BLK;
+            s.blk[j] = tile_block(t, min(k + j, k1 - 1));
+            s.page[j] = table[s.blk[j] >> shift];
         }
         return s;
     };
-    auto stage = [&](const Step& s, int buf) __attribute__((always_inline)) {
-        char* base = pf_lds + buf * (4 * BLK);
+    auto settle = [&](Step s) __attribute__((always_inline)) {
 #pragma unroll
         for (int j = 0; j < 2; j++) {
-            const __amdgpu_buffer_rsrc_t kr = coh_rsrc((const char*)a.pool.k + s.off[j] * (BLK / PAGE_BLK));
-            const __amdgpu_buffer_rsrc_t vr = coh_rsrc((const char*)a.pool.v + s.off[j] * (BLK / PAGE_BLK));
-#pragma unroll
-            for (int i = 0; i < KIB / PF_WAVES + (KIB % PF_WAVES != 0); i++) {
-                const int p = i * PF_WAVES + wid;
-                if (KIB % PF_WAVES && p >= KIB) break;
-                lds_dma16(kr, base + j * BLK + p * 1024, lane * 16, p * 1024);
-                lds_dma16(vr, base + (2 + j) * BLK + p * 1024, v_src, p * 1024);
-            }
+            const int p = __builtin_amdgcn_readfirstlane(s.page[j]);
+            s.page[j] = (unsigned)p < (unsigned)a.pool.n_pages ? p : -1;
         }
+        return s;
+    };
+    // first token of a block in the pool's arrays of tokens
+    auto token_of = [&](int blk, int page) __attribute__((always_inline)) {
+        return ((((size_t)max(page, 0) * a.pool.n_kv + t.kvh) << shift) + (blk & ((1 << shift) - 1))) * PAGE_BLK;
+    };
+    // wave w loads the keys (w < 2) or values of block w % 2 of a step
+    const int my_j = wid & 1, my_v = wid >> 1;
+    const char* my_pool = (const char*)(my_v ? a.pool.v : a.pool.k);
+    const int my_src = my_v ? v_src : lane * 16;
+    auto stage = [&](const Step& s, int buf) __attribute__((always_inline)) {
+        const size_t at = my_j ? token_of(s.blk[1], s.page[1]) : token_of(s.blk[0], s.page[0]);
+        const __amdgpu_buffer_rsrc_t rs = coh_rsrc(my_pool + at * (BLK / PAGE_BLK));
+        char* dst = pf_lds + buf * (4 * BLK) + (2 * my_v + my_j) * BLK;
+#pragma unroll
+        for (int i = 0; i < KIB; i += KIB < 4 ? KIB : 4) lds_dma_kib<KIB < 4 ? KIB : 4>(rs, dst + i * 1024, my_src, i * 1024);
     };
 
     float mx_run = -INFINITY, l = 0.f;
@@ -605,41 +662,39 @@ __global__ __launch_bounds__(PF_WAVES * 64, 2) void paged_prompt_kernel(PagedAtt
     for (int d = 0; d < DT; d++)
 #pragma unroll
         for (int i = 0; i < 16; i++) o[d][i] = 0.f;
-    bool bad = false;
-    Step cur{}, nxt{};
-    if (k0 < k1) {
-        nxt = step_at(k0);
-        stage(nxt, 0);
-    }
-    for (int k = k0, buf = 0; k < k1; k += 2, buf ^= 1) {
-        cur = nxt;
-        wait_vmcnt<0>();
-        __syncthreads();  // this step has landed for every wave, and the other stage is free
-        if (k + 2 < k1) {
-            nxt = step_at(k + 2);
-            stage(nxt, buf ^ 1);
+    const int wlow = a.window ? max(0, w_lo - a.window + 1) : 0;
+
+    // A step of this wave in two parts.  MASK: the general form.  Without MASK every row of the tile sees every token.
+    struct Work {
+        float16_t s[2];             // scores, then weights
+        float vsc[2][I8 ? 16 : 1];  // INT8: scales of V
+        float mx;                   // largest exponent of the column
+        bool skip[2];               // blocks that no row of this wave sees
+    };
+    auto factor = [&](auto mask) { return (!mask.value && MODE == 1) || MODE == 0 ? qs * PA_LOG2E : 1.f; };
+    auto scores = [&](const Step& cur, int buf, bool two, auto mask, Work& w) __attribute__((always_inline)) {
+        constexpr bool MASK = mask.value;
+        constexpr bool direct = !MASK && MODE == 1;
+        const float c = factor(mask);
+        float16_t(&s)[2] = w.s;
+        auto& vsc = w.vsc;
+        const int t0[2] = {cur.blk[0] * PAGE_BLK, cur.blk[1] * PAGE_BLK};
+        w.skip[0] = w.skip[1] = false;
+        if constexpr (MASK) {
+#pragma unroll
+            for (int j = 0; j < 2; j++)
+                w.skip[j] = (j && !two) || cur.page[j] < 0 || (t0[j] >= t.pre && (t0[j] > w_hi || t0[j] + PAGE_BLK <= wlow));
+            if (idle || (w.skip[0] && w.skip[1])) return false;
         }
-        const bool two = k + 1 < k1;
-        bad |= cur.page[0] < 0 || (two && cur.page[1] < 0);
-        // blocks that no row of this wave sees
-        auto unseen = [&](int t0) { return t0 > w_hi && t0 >= t.pre; };
-        const int wlow = a.window ? max(0, w_lo - a.window + 1) : 0;
-        auto before = [&](int t0) { return t0 + PAGE_BLK <= wlow && t0 >= t.pre; };
-        const bool skip0 = cur.page[0] < 0 || unseen(cur.t0[0]) || before(cur.t0[0]);
-        const bool skip1 = !two || cur.page[1] < 0 || unseen(cur.t0[1]) || before(cur.t0[1]);
-        if (idle || (skip0 && skip1)) continue;
         const char* kb = pf_lds + buf * (4 * BLK) + k_lane;
-        const char* vb = pf_lds + buf * (4 * BLK) + 2 * BLK;
-        float16_t s[2];
+        s[0] = s[1] = float16_t{};
+        if constexpr (I8) {
 #pragma unroll
-        for (int j = 0; j < 2; j++) {
+            for (int c = 0; c < KS / 4; c++)
 #pragma unroll
-            for (int i = 0; i < 16; i++) s[j][i] = 0.f;
-            if constexpr (I8) {
+                for (int g = 0; g < 2; g++)
 #pragma unroll
-                for (int c = 0; c < KS / 4; c++)
-#pragma unroll
-                    for (int g = 0; g < 2; g++) {
+                    for (int j = 0; j < 2; j++) {
                         const u32x4_t w = *(const u32x4_t*)(kb + j * BLK + c * 1024 + g * 512);
 #pragma unroll
                         for (int half = 0; half < 2; half++) {
@@ -649,65 +704,63 @@ __global__ __launch_bounds__(PF_WAVES * 64, 2) void paged_prompt_kernel(PagedAtt
                             if constexpr (F32) s[j] = mfma32<KVF>(ka, ql[ks], s[j]);
                         }
                     }
-            } else {
+        } else {
 #pragma unroll
-                for (int ks = 0; ks < KS; ks++) {
+            for (int ks = 0; ks < KS; ks++)
+#pragma unroll
+                for (int j = 0; j < 2; j++) {
                     const frag ka = *(const frag*)(kb + j * BLK + (ks >> 1) * 1024 + (ks & 1) * 512);
                     s[j] = mfma32<KVF>(ka, qh[ks], s[j]);
                     if constexpr (F32) s[j] = mfma32<KVF>(ka, ql[ks], s[j]);
                 }
-            }
         }
-        auto whole_at = [&](int t0) {
-            return t0 + PAGE_BLK - 1 <= w_lo && (a.window == 0 || t0 > w_hi - a.window || t0 + PAGE_BLK <= t.pre);
-        };
-        const bool whole = !skip0 && !skip1 && whole_at(cur.t0[0]) && whole_at(cur.t0[1]);
-        float vsc[2][I8 ? 16 : 1];
         float vexp = 0.f;
         if constexpr (I8) {
             float top = 0.f;
 #pragma unroll
-            for (int j = 0; j < 2; j++)
+            for (int j = 0; j < 2; j++) {
+                const size_t at = token_of(cur.blk[j], cur.page[j]) + 8 * hk;
 #pragma unroll
                 for (int g = 0; g < 2; g++) {
-                    const half8_t ksc = *(const half8_t*)(a.pool.ks + cur.off[j] + 16 * g + 8 * hk);
-                    const half8_t vs = *(const half8_t*)(a.pool.vs + cur.off[j] + 16 * g + 8 * hk);
+                    const half8_t ksc = *(const half8_t*)(a.pool.ks + at + 16 * g);
+                    const half8_t vs = *(const half8_t*)(a.pool.vs + at + 16 * g);
 #pragma unroll
                     for (int i = 0; i < 8; i++) {
                         s[j][8 * g + i] *= (float)ksc[i];
                         const float v = (float)vs[i];
                         vsc[j][8 * g + i] = v;
-                        top = fmaxf(top, cur.t0[j] + 16 * g + 8 * hk + i < t.s.kv_len ? v : 0.f);
+                        top = fmaxf(top, !MASK || t0[j] + 16 * g + 8 * hk + i < t.s.kv_len ? v : 0.f);
                     }
                 }
+            }
             top = half_max(top);
             vexp = top > 0x1p-20f ? (float)__builtin_amdgcn_frexp_expf(top) : -20.f;
         }
-        if (plain) {
-            const float c = qs * PA_LOG2E;
+        // scores to powers of two: exponent = s * c - ref.  A capped score whose block needs no mask goes
+        // from the product to the weight in one go further down.
+        if constexpr (MODE != 0) if (!direct) {
 #pragma unroll
-            for (int j = 0; j < 2; j++)
-#pragma unroll
-                for (int i = 0; i < 16; i++) s[j][i] *= c;
-        } else {
-#pragma unroll
-            for (int j = 0; j < 2; j++)
+            for (int j = 0; j < 2; j++) {
+                const float at = slope * (float)(t0[j] + 8 * hk - pos);
 #pragma unroll
                 for (int i = 0; i < 16; i++) {
                     float x = s[j][i] * qs;
-                    if (a.softcap > 0.f) x = a.softcap * tanh_f32(x / a.softcap);
-                    s[j][i] = x * PA_LOG2E + slope * (float)(cur.t0[j] + 16 * (i >> 3) + 8 * hk + (i & 7) - pos);
+                    if (MODE == 1 || capped) x = a.softcap * tanh_f32<F32>(x * inv_cap);
+                    s[j][i] = fmaf(x, PA_LOG2E, fmaf(slope, (float)(16 * (i >> 3) + (i & 7)), at));
                 }
+            }
         }
-        if (!whole) {
+        if constexpr (MASK) {
 #pragma unroll
-            for (int j = 0; j < 2; j++)
+            for (int j = 0; j < 2; j++) {
+                // visible tokens of the block as bits: low .. pos, and those of the prefix
+                const int base = t0[j] + 8 * hk, low = a.window ? pos - a.window + 1 : 0;
+                const int hi_n = min(max(pos + 1 - base, 0), 32), lo_n = min(max(low - base, 0), 32), pre_n = min(max(t.pre - base, 0), 32);
+                auto ones = [](int n) { return n >= 32 ? 0xFFFFFFFFu : (1u << n) - 1u; };
+                const uint32_t seen = w.skip[j] ? 0u : (ones(hi_n) & ~ones(lo_n)) | ones(pre_n);
 #pragma unroll
-                for (int i = 0; i < 16; i++) {
-                    const int tk = cur.t0[j] + 16 * (i >> 3) + 8 * hk + (i & 7);
-                    const bool seen = !(j ? skip1 : skip0) && ((tk <= pos && (a.window == 0 || pos - tk < a.window)) || tk < t.pre);
-                    s[j][i] = seen ? s[j][i] : -INFINITY;
-                }
+                for (int i = 0; i < 16; i++) s[j][i] = (seen >> (16 * (i >> 3) + (i & 7))) & 1u ? s[j][i] : -INFINITY;
+            }
         }
         float mx = s[0][0];
 #pragma unroll
@@ -715,64 +768,144 @@ __global__ __launch_bounds__(PF_WAVES * 64, 2) void paged_prompt_kernel(PagedAtt
 #pragma unroll
         for (int i = 0; i < 16; i++) mx = fmaxf(mx, s[1][i]);
         mx = half_max(mx);
+        mx = direct ? cap2 * tanh_f32<F32>(mx * qs * inv_cap) : mx * c;
         if constexpr (I8) mx += vexp;
+        w.mx = mx;
+        return true;
+    };
+    // O's reference follows the maximum
+    auto raise = [&](float mx) __attribute__((always_inline)) {
         const float mn = fmaxf(mx_run, mx);
-        if (__any(mn > mx_run)) {
-            const float alpha = mn == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(mx_run - mn);
-            l *= alpha;
+        const float alpha = mn == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(mx_run - mn);
+        l *= alpha;
 #pragma unroll
-            for (int d = 0; d < DT; d++) o[d] *= alpha;
-            mx_run = mn;
+        for (int d = 0; d < DT; d++) o[d] *= alpha;
+        mx_run = mn;
+    };
+    auto add = [&](const Step& cur, int buf, auto mask, Work& w) __attribute__((always_inline)) {
+        constexpr bool MASK = mask.value;
+        constexpr bool direct = !MASK && MODE == 1;
+        const float c = factor(mask);
+        float16_t(&s)[2] = w.s;
+        auto& vsc = w.vsc;
+        const int t0[2] = {cur.blk[0] * PAGE_BLK, cur.blk[1] * PAGE_BLK};
+        const char* vb = pf_lds + buf * (4 * BLK) + 2 * BLK;
+        const float ref = (mx_run == -INFINITY ? 0.f : mx_run) - Mat<KVF>::P_BITS;
+        if constexpr (direct) {
+            const float k2 = 2.f * c * inv_cap;
+#pragma unroll
+            for (int j = 0; j < 2; j++)
+#pragma unroll
+                for (int i = 0; i < 16; i++) {
+                    if constexpr (F32) s[j][i] = __builtin_amdgcn_exp2f(cap2 * tanh_f32<true>(s[j][i] * qs * inv_cap) - ref);
+                    else s[j][i] = __builtin_amdgcn_exp2f(-2.f * cap2 * __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(s[j][i] * k2) + 1.f) + (cap2 - ref));
+                }
+        } else {
+#pragma unroll
+            for (int j = 0; j < 2; j++)
+#pragma unroll
+                for (int i = 0; i < 16; i++) s[j][i] = __builtin_amdgcn_exp2f(fmaf(s[j][i], c, -ref));
         }
-        const float ref = (mn == -INFINITY ? 0.f : mn) - Mat<KVF>::P_BITS;
-        frag ph[2][2], pl[F32 ? 2 : 1][2];
 #pragma unroll
         for (int j = 0; j < 2; j++)
 #pragma unroll
-            for (int i = 0; i < 16; i++) {
-                float p = __builtin_amdgcn_exp2f(s[j][i] - ref);
-                l += p;
-                if constexpr (I8) p = s[j][i] == -INFINITY ? 0.f : p * vsc[j][i];
-                ph[j][i >> 3][i & 7] = (elem)p;
-                if constexpr (F32) pl[j][i >> 3][i & 7] = (elem)(p - (float)ph[j][i >> 3][i & 7]);
-            }
-#pragma unroll
-        for (int j = 0; j < 2; j++) {
-#pragma unroll
             for (int g = 0; g < 2; g++) {
+                frag ph, pl;
+#pragma unroll
+                for (int i = 0; i < 8; i++) {
+                    float p = s[j][8 * g + i];
+                    l += p;
+                    if constexpr (I8) {
+                        // a token that is not there may have any scale
+                        p = MASK && p == 0.f ? 0.f : p * vsc[j][8 * g + i];
+                    }
+                    ph[i] = (elem)p;
+                    if constexpr (F32) pl[i] = (elem)(p - (float)ph[i]);
+                }
                 u32x4_t keep;
-                if constexpr (!I8) {
+                if constexpr (MASK && !I8) {
                     // tokens that no row of this wave sees may hold anything, also NaN
-                    if (!whole) {
+                    const int base = t0[j] + 16 * g + 8 * hk;
 #pragma unroll
-                        for (int i = 0; i < 4; i++) {
-                            uint32_t w = 0;
+                    for (int i = 0; i < 4; i++) {
+                        uint32_t kw = 0;
 #pragma unroll
-                            for (int e = 0; e < 2; e++) {
-                                const int tk = cur.t0[j] + 16 * g + 8 * hk + 2 * i + e;
-                                const bool any = !(j ? skip1 : skip0) && ((tk <= w_hi && tk >= wlow) || tk < t.pre);
-                                w |= any ? 0xFFFFu << (16 * e) : 0u;
-                            }
-                            keep[i] = w;
+                        for (int e = 0; e < 2; e++) {
+                            const int tk = base + 2 * i + e;
+                            const bool any = !w.skip[j] & (((tk <= w_hi) & (tk >= wlow)) | (tk < t.pre));
+                            kw |= any ? 0xFFFFu << (16 * e) : 0u;
                         }
+                        keep[i] = kw;
                     }
                 }
 #pragma unroll
                 for (int d = 0; d < DT; d++) {
                     frag va;
                     if constexpr (I8) {
-                        const uint2 w = *(const uint2*)(vb + j * BLK + v_lane + d * 1024 + g * 512);
-                        va = i8_to_half8(w.x, w.y);
+                        const uint2 vw = *(const uint2*)(vb + j * BLK + v_lane + d * 1024 + g * 512);
+                        va = i8_to_half8(vw.x, vw.y);
                     } else {
-                        u32x4_t w = *(const u32x4_t*)(vb + j * BLK + (v_lane ^ (g * 32)) + d * 2048);
-                        if (!whole) w &= keep;
-                        va = __builtin_bit_cast(frag, w);
+                        u32x4_t vw = *(const u32x4_t*)(vb + j * BLK + (v_lane ^ (g * 32)) + d * 2048);
+                        if constexpr (MASK) vw &= keep;
+                        va = __builtin_bit_cast(frag, vw);
                     }
-                    o[d] = mfma32<KVF>(va, ph[j][g], o[d]);
-                    if constexpr (F32) o[d] = mfma32<KVF>(va, pl[j][g], o[d]);
+                    o[d] = mfma32<KVF>(va, ph, o[d]);
+                    if constexpr (F32) o[d] = mfma32<KVF>(va, pl, o[d]);
                 }
             }
+    };
+
+    bool bad = false;
+    Step cur{}, nxt{}, far{};
+    if (k0 < k1) {
+        nxt = settle(look_up(k0));
+        far = look_up(k0 + 2);
+        stage(nxt, 0);
+    }
+    const int whole_lo = a.window ? t.p_hi - a.window + 1 : 0;  // tokens from here to p_lo are seen by every row
+    const bool full = t.r0 + PF_ROWS <= rows;
+    int k = k0, buf = 0;
+    // next step: its data has landed for every wave, and the other stage is free for the one after it
+    auto advance = [&]() __attribute__((always_inline)) {
+        cur = nxt;
+        wait_vmcnt<0>();
+        __syncthreads();
+        if (k + 2 < k1) {
+            nxt = settle(far);
+            far = look_up(k + 4);
+            stage(nxt, buf ^ 1);
         }
+    };
+    auto whole = [&](const Step& s) {
+        return full & (k + 1 < k1) & (s.page[0] >= 0) & (s.page[1] >= 0) & (s.blk[1] * PAGE_BLK + PAGE_BLK - 1 <= t.p_lo) &
+               (s.blk[0] * PAGE_BLK >= whole_lo);
+    };
+    for (;;) {
+        // Steps that need no mask, while the maximum stays: nothing in this loop touches O but the products, and it
+        // keeps its registers (a conditional factor cost 64 copies a step).
+        bool landed = false;
+        while (whole(nxt)) {
+            advance();
+            Work w;
+            scores(cur, buf, true, std::false_type{}, w);
+            landed = __any(w.mx > mx_run + Mat<KVF>::P_LAG);
+            if (landed) break;  // made again below
+            add(cur, buf, std::false_type{}, w);
+            k += 2;
+            buf ^= 1;
+        }
+        if (!landed) {
+            if (k >= k1) break;
+            advance();
+        }
+        bad |= cur.page[0] < 0 || cur.page[1] < 0;
+        Work w;
+        if (scores(cur, buf, k + 1 < k1, std::true_type{}, w)) {
+            if (__any(w.mx > mx_run + Mat<KVF>::P_LAG)) raise(w.mx);
+            add(cur, buf, std::true_type{}, w);
+        }
+        k += 2;
+        buf ^= 1;
     }
     if (bad && a.bt.status && tid == 0) atomicOr(&a.bt.status[t.b], PAGE_SEQ_BAD_PAGE);
     l = half_sum(l);
@@ -841,7 +974,10 @@ int launch_hd(const PagedAttnArgs& a, hipStream_t stream) {
     auto go = [&](auto kernel, unsigned lds) {
         hipLaunchKernelGGL(kernel, grid, dim3(256), lds, stream, a, group, p.tiles, p.splits, p.per);
     };
-    if (p.prompt) go(paged_prompt_kernel<T, KVF, HD>, 8 * PAGE_BLK * HD * (KVF == KV_INT8 ? 1 : 2));
+    const unsigned lds = 8 * PAGE_BLK * HD * (KVF == KV_INT8 ? 1 : 2);
+    if (p.prompt && a.slopes) go(paged_prompt_kernel<T, KVF, HD, 2>, lds);
+    else if (p.prompt && a.softcap > 0.f) go(paged_prompt_kernel<T, KVF, HD, 1>, lds);
+    else if (p.prompt) go(paged_prompt_kernel<T, KVF, HD, 0>, lds);
     else if (p.nt == 1) go(paged_decode_kernel<T, KVF, HD, 1>, 0);
     else go(paged_decode_kernel<T, KVF, HD, 2>, 0);
     if (p.splits > 1) {
