@@ -11,6 +11,7 @@
 // (2^-11 or 2^-8 of each weight, as V itself was); f32 queries are split into fp16 hi + lo
 // halves, and so is P (2^-22 together): two matrix instructions in place of one.
 #include <algorithm>
+#include <cmath>
 #include <type_traits>
 
 #include "device_common.hpp"
@@ -134,10 +135,13 @@ __device__ __forceinline__ float2_t* part_ml(const PagedAttnArgs& a, int splits,
 // ---------------------------------------------------------------------------
 // Few rows: the cache is streamed through the registers
 // ---------------------------------------------------------------------------
-constexpr int DC_WAVES = 4;
+// Waves of a workgroup, which share its blocks one by one.  INT8 blocks need more arithmetic for their bytes, and a second
+// wave on each SIMD (32 x 4 rows over 4096 tokens 52 us, 76 with four waves); 16-bit pools stream as
+// well with four (64 x 1 over 4096 6.3 TB/s either way) and have less to join.
+constexpr int dc_waves(int kvf) { return kvf == KV_INT8 ? 8 : 4; }
 
 template <typename T, int KVF, int HD, int NT>
-__global__ __launch_bounds__(DC_WAVES * 64, 2) void paged_decode_kernel(PagedAttnArgs a, int group, int tiles, int splits, int per) {
+__global__ __launch_bounds__(dc_waves(KVF) * 64) void paged_decode_kernel(PagedAttnArgs a, int group, int tiles, int splits, int per) {
     typedef typename Mat<KVF>::frag frag;
     typedef typename Mat<KVF>::elem elem;
     constexpr bool I8 = KVF == KV_INT8, F32 = std::is_same<T, float>::value;
@@ -146,6 +150,7 @@ __global__ __launch_bounds__(DC_WAVES * 64, 2) void paged_decode_kernel(PagedAtt
     constexpr int KL = I8 ? HD / 32 : HD / 16;  // 16-byte pieces of a lane's share of a K (or V) block
     constexpr int BLK = PAGE_BLK * HD * (I8 ? 1 : 2);
     constexpr int LDO = HD + 4;
+    constexpr int DC_WAVES = dc_waves(KVF);
     __shared__ float s_o[DC_WAVES][16 * LDO];
     __shared__ float2_t s_ml[DC_WAVES][16];
     const int tid = threadIdx.x, lane = tid & 63, wid = __builtin_amdgcn_readfirstlane(tid >> 6), lr = lane & 15, lg = lane >> 4;
@@ -441,39 +446,57 @@ __global__ __launch_bounds__(DC_WAVES * 64, 2) void paged_decode_kernel(PagedAtt
                 if (d == 0) *part_ml(a, splits, split, slot) = float2_t{M, L};
             } else {
                 const float inv = L > 0.f ? 1.f / L : 0.f;
-                T* out = (T*)a.out + (long long)(t.s.row0 + tok) * a.out_ld + (long long)h * HD + d;
-#pragma unroll
-                for (int j = 0; j < 4; j++) out[j] = (T)(acc[j] * inv);
+                typedef T out4 __attribute__((ext_vector_type(4)));
+                *(out4*)((T*)a.out + (long long)(t.s.row0 + tok) * a.out_ld + (long long)h * HD + d) =
+                    out4{(T)(acc[0] * inv), (T)(acc[1] * inv), (T)(acc[2] * inv), (T)(acc[3] * inv)};
             }
         }
     }
 }
 
-// Joins the splits of a call: HD / 4 threads per (row, head).
+// Joins the splits of a call: one wave per (row, head).  Lane k holds split k's (maximum, sum); HD / 4 lanes take one
+// split's sums at a time, so a wave has 2 (HD 128) or 4 splits in hand at once.
 template <typename T, int HD>
 __global__ __launch_bounds__(256) void paged_merge_kernel(PagedAttnArgs a, int splits) {
-    const int b = blockIdx.y;
+    constexpr int LN = HD / 4, PAR = 64 / LN;
+    const int b = blockIdx.y, lane = threadIdx.x & 63, part = lane / LN, d = lane % LN * 4;
     PageSeq s;
     if (!page_seq(a.bt.row_off, a.bt.kv_len, b, a.bt.rows, a.bt.max_rows, a.bt.max_kv, &s)) return;
-    const long long i = (long long)blockIdx.x * 256 + threadIdx.x;
-    const long long at = i / (HD / 4);
-    const int d = (int)(i % (HD / 4)) * 4;
+    const long long at = (long long)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     if (at >= (long long)s.rows * a.n_heads) return;
     const long long slot = (long long)s.row0 * a.n_heads + at;
-    float M = -INFINITY;
-    for (int k = 0; k < splits; k++) M = fmaxf(M, (*part_ml(a, splits, k, slot))[0]);
-    float L = 0.f;
-    float4_t acc = {0.f, 0.f, 0.f, 0.f};
-    for (int k = 0; k < splits; k++) {
-        const float2_t ml = *part_ml(a, splits, k, slot);
-        const float f = ml[0] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(ml[0] - M);
-        L += ml[1] * f;
-        acc += *(const float4_t*)(part_o(a, k, slot) + d) * f;
-    }
-    const float inv = L > 0.f ? 1.f / L : 0.f;
-    T* out = (T*)a.out + (s.row0 + at / a.n_heads) * a.out_ld + (at % a.n_heads) * HD + d;
+    float2_t ml = {-INFINITY, 0.f};
+    if (lane < splits) ml = *part_ml(a, splits, lane, slot);
+    constexpr int AHEAD = 4;  // loads in flight a lane
+    float4_t v[AHEAD];
 #pragma unroll
-    for (int j = 0; j < 4; j++) out[j] = (T)(acc[j] * inv);
+    for (int i = 0; i < AHEAD; i++) {
+        const int k = i * PAR + part;
+        if (k < splits) v[i] = *(const float4_t*)(part_o(a, k, slot) + d);
+    }
+    const float M = wave_max_f32(ml[0]);
+    const float f = ml[0] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(ml[0] - M);
+    const float L = wave_sum_f32(ml[1] * f);
+    float4_t acc = {0.f, 0.f, 0.f, 0.f};
+    for (int k0 = 0; k0 < splits; k0 += AHEAD * PAR) {
+#pragma unroll
+        for (int i = 0; i < AHEAD; i++) {
+            const int k = k0 + i * PAR + part;
+            const float fk = __shfl(f, k & 63);
+            if (k < splits) acc += v[i] * fk;
+            const int kn = k + AHEAD * PAR;
+            if (kn < splits) v[i] = *(const float4_t*)(part_o(a, kn, slot) + d);
+        }
+    }
+#pragma unroll
+    for (int x = LN; x < 64; x *= 2)
+#pragma unroll
+        for (int j = 0; j < 4; j++) acc[j] += __shfl_xor(acc[j], x);
+    if (part) return;
+    const float inv = L > 0.f ? 1.f / L : 0.f;
+    typedef T out4 __attribute__((ext_vector_type(4)));
+    *(out4*)((T*)a.out + (s.row0 + at / a.n_heads) * a.out_ld + (at % a.n_heads) * HD + d) =
+        out4{(T)(acc[0] * inv), (T)(acc[1] * inv), (T)(acc[2] * inv), (T)(acc[3] * inv)};
 }
 
 // ---------------------------------------------------------------------------
@@ -500,38 +523,6 @@ __device__ __forceinline__ float half_sum(float x) {
     return __uint_as_float(b[0]) + __uint_as_float(b[1]);
 }
 
-// N consecutive KiB (global and LDS) in one go, as lds_dma16 (the instruction offset moves both addresses).
-template <int N>
-__device__ __forceinline__ void lds_dma_kib(__amdgpu_buffer_rsrc_t r, const void* lds_dst, int voff, int soff) {
-    static_assert(N == 2 || N == 4, "two or four KiB");
-    const unsigned base = __builtin_amdgcn_readfirstlane((unsigned)(uintptr_t)lds_dst);
-    int saved;
-    if constexpr (N == 2)
-        asm volatile(
-            "s_mov_b32 %0, m0\n\t"
-            "s_mov_b32 m0, %1\n\t"
-            "s_nop 0\n\t"
-            "buffer_load_dwordx4 %2, %3, %4 offen lds\n\t"
-            "buffer_load_dwordx4 %2, %3, %4 offen offset:1024 lds\n\t"
-            "s_mov_b32 m0, %0"
-            : "=&s"(saved)
-            : "s"(base), "v"(voff), "s"(r), "s"(soff)
-            : "memory");
-    else
-        asm volatile(
-            "s_mov_b32 %0, m0\n\t"
-            "s_mov_b32 m0, %1\n\t"
-            "s_nop 0\n\t"
-            "buffer_load_dwordx4 %2, %3, %4 offen lds\n\t"
-            "buffer_load_dwordx4 %2, %3, %4 offen offset:1024 lds\n\t"
-            "buffer_load_dwordx4 %2, %3, %4 offen offset:2048 lds\n\t"
-            "buffer_load_dwordx4 %2, %3, %4 offen offset:3072 lds\n\t"
-            "s_mov_b32 m0, %0"
-            : "=&s"(saved)
-            : "s"(base), "v"(voff), "s"(r), "s"(soff)
-            : "memory");
-}
-
 constexpr int PF_WAVES = 4, PF_ROWS = 32 * PF_WAVES;
 
 // MODE 0: scores as they are, 1: capped, 2: a slope per head (capped or not)
@@ -544,7 +535,7 @@ __global__ __launch_bounds__(PF_WAVES * 64, 2) void paged_prompt_kernel(PagedAtt
     constexpr int DT = HD / 32;  // 32-dimension tiles of O^T
     constexpr int BLK = PAGE_BLK * HD * (I8 ? 1 : 2);
     constexpr int KIB = BLK / 1024;  // wave loads of a block of K (or V)
-    extern __shared__ char pf_lds[];  // [2 stages][K: 2 blocks | V: 2 blocks]
+    __shared__ __attribute__((aligned(1024))) char pf_lds[8 * BLK];  // [2 stages][K: 2 blocks | V: 2 blocks]
     const int tid = threadIdx.x, lane = tid & 63, wid = __builtin_amdgcn_readfirstlane(tid >> 6), hk = lane >> 5, m = lane & 31;
     int id = blockIdx.x;
     const int pairs = a.bt.nseq * a.pool.n_kv;
@@ -557,6 +548,7 @@ __global__ __launch_bounds__(PF_WAVES * 64, 2) void paged_prompt_kernel(PagedAtt
     const int rows = t.s.rows * group, pos0 = t.s.kv_len - t.s.rows;
 
     // this lane's query
+    // (columns past the last row repeat it, and are not stored)
     const int r = t.r0 + wid * 32 + m, rr = min(r, rows - 1), tok = rr / group;
     const int h = head_of(a, t.kvh, rr - tok * group, group);
     const int pos = pos0 + tok;
@@ -648,12 +640,24 @@ __global__ __launch_bounds__(PF_WAVES * 64, 2) void paged_prompt_kernel(PagedAtt
     const int my_j = wid & 1, my_v = wid >> 1;
     const char* my_pool = (const char*)(my_v ? a.pool.v : a.pool.k);
     const int my_src = my_v ? v_src : lane * 16;
-    auto stage = [&](const Step& s, int buf) __attribute__((always_inline)) {
+    // ... one KiB at a time: pieces of the next step's loads go between this step's products (issued in a row they
+    // hold the wave until the address unit has taken them: 1000 cycles of a step)
+    struct Load {
+        uint32_t lo, hi;  // global address of the block
+        char* dst;
+    };
+    auto load_of = [&](const Step& s, int buf) __attribute__((always_inline)) {
         const size_t at = my_j ? token_of(s.blk[1], s.page[1]) : token_of(s.blk[0], s.page[0]);
-        const __amdgpu_buffer_rsrc_t rs = coh_rsrc(my_pool + at * (BLK / PAGE_BLK));
-        char* dst = pf_lds + buf * (4 * BLK) + (2 * my_v + my_j) * BLK;
+        const uint64_t p = (uint64_t)(my_pool + at * (BLK / PAGE_BLK));
+        return Load{(uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)p), (uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)(p >> 32)),
+                    pf_lds + buf * (4 * BLK) + (2 * my_v + my_j) * BLK};
+    };
+    auto piece = [&](const Load& ld, int i) __attribute__((always_inline)) {
+        lds_dma16(coh_rsrc((const void*)(((uint64_t)ld.hi << 32) | ld.lo)), ld.dst + i * 1024, my_src, i * 1024);
+    };
+    auto pieces = [&](const Load& ld) __attribute__((always_inline)) {
 #pragma unroll
-        for (int i = 0; i < KIB; i += KIB < 4 ? KIB : 4) lds_dma_kib<KIB < 4 ? KIB : 4>(rs, dst + i * 1024, my_src, i * 1024);
+        for (int i = 0; i < KIB; i++) piece(ld, i);
     };
 
     float mx_run = -INFINITY, l = 0.f;
@@ -672,7 +676,7 @@ __global__ __launch_bounds__(PF_WAVES * 64, 2) void paged_prompt_kernel(PagedAtt
         bool skip[2];               // blocks that no row of this wave sees
     };
     auto factor = [&](auto mask) { return (!mask.value && MODE == 1) || MODE == 0 ? qs * PA_LOG2E : 1.f; };
-    auto scores = [&](const Step& cur, int buf, bool two, auto mask, Work& w) __attribute__((always_inline)) {
+    auto scores = [&](const Step& cur, int buf, bool two, const Load* ld, auto mask, Work& w) __attribute__((always_inline)) {
         constexpr bool MASK = mask.value;
         constexpr bool direct = !MASK && MODE == 1;
         const float c = factor(mask);
@@ -688,31 +692,38 @@ __global__ __launch_bounds__(PF_WAVES * 64, 2) void paged_prompt_kernel(PagedAtt
         }
         const char* kb = pf_lds + buf * (4 * BLK) + k_lane;
         s[0] = s[1] = float16_t{};
-        if constexpr (I8) {
+        // operands are read two iterations before their products
+        constexpr int QN = I8 ? KS / 2 : KS;  // iterations; INT8 operands are two k-steps each
+        static_assert(QN == KIB, "one piece of the next step an iteration");
+        u32x4_t ka[3][2];
+        auto read = [&](int i) __attribute__((always_inline)) {
 #pragma unroll
-            for (int c = 0; c < KS / 4; c++)
+            for (int j = 0; j < 2; j++) ka[i % 3][j] = *(const u32x4_t*)(kb + j * BLK + (i >> 1) * 1024 + (i & 1) * 512);
+        };
+        read(0);
+        if (QN > 1) read(1);
 #pragma unroll
-                for (int g = 0; g < 2; g++)
+        for (int i = 0; i < QN; i++) {
+            if (i + 2 < QN) read(i + 2);
+            if constexpr (!MASK) piece(*ld, i);
 #pragma unroll
-                    for (int j = 0; j < 2; j++) {
-                        const u32x4_t w = *(const u32x4_t*)(kb + j * BLK + c * 1024 + g * 512);
+            for (int j = 0; j < 2; j++) {
+                const u32x4_t kw = ka[i % 3][j];
+                if constexpr (I8) {
 #pragma unroll
-                        for (int half = 0; half < 2; half++) {
-                            const half8_t ka = half ? i8_to_half8(w[2], w[3]) : i8_to_half8(w[0], w[1]);
-                            const int ks = c * 4 + half * 2 + g;
-                            s[j] = mfma32<KVF>(ka, qh[ks], s[j]);
-                            if constexpr (F32) s[j] = mfma32<KVF>(ka, ql[ks], s[j]);
-                        }
+                    for (int half = 0; half < 2; half++) {
+                        const half8_t kf = half ? i8_to_half8(kw[2], kw[3]) : i8_to_half8(kw[0], kw[1]);
+                        const int ks = (i >> 1) * 4 + half * 2 + (i & 1);
+                        s[j] = mfma32<KVF>(kf, qh[ks], s[j]);
+                        if constexpr (F32) s[j] = mfma32<KVF>(kf, ql[ks], s[j]);
                     }
-        } else {
-#pragma unroll
-            for (int ks = 0; ks < KS; ks++)
-#pragma unroll
-                for (int j = 0; j < 2; j++) {
-                    const frag ka = *(const frag*)(kb + j * BLK + (ks >> 1) * 1024 + (ks & 1) * 512);
-                    s[j] = mfma32<KVF>(ka, qh[ks], s[j]);
-                    if constexpr (F32) s[j] = mfma32<KVF>(ka, ql[ks], s[j]);
+                } else {
+                    const frag kf = __builtin_bit_cast(frag, kw);
+                    s[j] = mfma32<KVF>(kf, qh[i], s[j]);
+                    if constexpr (F32) s[j] = mfma32<KVF>(kf, ql[i], s[j]);
                 }
+            }
+            if constexpr (!MASK) __builtin_amdgcn_sched_barrier(0);  // in this order
         }
         float vexp = 0.f;
         if constexpr (I8) {
@@ -853,6 +864,16 @@ __global__ __launch_bounds__(PF_WAVES * 64, 2) void paged_prompt_kernel(PagedAtt
                     if constexpr (F32) o[d] = mfma32<KVF>(va, pl, o[d]);
                 }
             }
+        if constexpr (!MASK && !I8) {
+            // V operands are read four products early (left alone, the compiler reads each just before its product)
+            __builtin_amdgcn_sched_group_barrier(0x100, 4, 0);
+#pragma unroll
+            for (int i = 0; i < 4 * DT - 4; i++) {
+                __builtin_amdgcn_sched_group_barrier(0x8, F32 ? 2 : 1, 0);
+                __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+            }
+            __builtin_amdgcn_sched_group_barrier(0x8, F32 ? 8 : 4, 0);
+        }
     };
 
     bool bad = false;
@@ -860,10 +881,9 @@ __global__ __launch_bounds__(PF_WAVES * 64, 2) void paged_prompt_kernel(PagedAtt
     if (k0 < k1) {
         nxt = settle(look_up(k0));
         far = look_up(k0 + 2);
-        stage(nxt, 0);
+        pieces(load_of(nxt, 0));
     }
     const int whole_lo = a.window ? t.p_hi - a.window + 1 : 0;  // tokens from here to p_lo are seen by every row
-    const bool full = t.r0 + PF_ROWS <= rows;
     int k = k0, buf = 0;
     // next step: its data has landed for every wave, and the other stage is free for the one after it
     auto advance = [&]() __attribute__((always_inline)) {
@@ -873,11 +893,11 @@ __global__ __launch_bounds__(PF_WAVES * 64, 2) void paged_prompt_kernel(PagedAtt
         if (k + 2 < k1) {
             nxt = settle(far);
             far = look_up(k + 4);
-            stage(nxt, buf ^ 1);
         }
+        return load_of(nxt, buf ^ 1);  // (the last step loads itself again: nobody reads that)
     };
     auto whole = [&](const Step& s) {
-        return full & (k + 1 < k1) & (s.page[0] >= 0) & (s.page[1] >= 0) & (s.blk[1] * PAGE_BLK + PAGE_BLK - 1 <= t.p_lo) &
+        return (k + 1 < k1) & (s.page[0] >= 0) & (s.page[1] >= 0) & (s.blk[1] * PAGE_BLK + PAGE_BLK - 1 <= t.p_lo) &
                (s.blk[0] * PAGE_BLK >= whole_lo);
     };
     for (;;) {
@@ -885,28 +905,29 @@ __global__ __launch_bounds__(PF_WAVES * 64, 2) void paged_prompt_kernel(PagedAtt
         // keeps its registers (a conditional factor cost 64 copies a step).
         bool landed = false;
         while (whole(nxt)) {
-            advance();
+            const Load ld = advance();
             Work w;
-            scores(cur, buf, true, std::false_type{}, w);
+            scores(cur, buf, true, &ld, std::false_type{}, w);
             landed = __any(w.mx > mx_run + Mat<KVF>::P_LAG);
             if (landed) break;  // made again below
             add(cur, buf, std::false_type{}, w);
             k += 2;
             buf ^= 1;
         }
-        if (!landed) {
+        if (!landed) {  // (otherwise the next step's pieces are on their way)
             if (k >= k1) break;
-            advance();
+            pieces(advance());
         }
         bad |= cur.page[0] < 0 || cur.page[1] < 0;
         Work w;
-        if (scores(cur, buf, k + 1 < k1, std::true_type{}, w)) {
+        if (scores(cur, buf, k + 1 < k1, nullptr, std::true_type{}, w)) {
             if (__any(w.mx > mx_run + Mat<KVF>::P_LAG)) raise(w.mx);
             add(cur, buf, std::true_type{}, w);
         }
         k += 2;
         buf ^= 1;
     }
+    wait_vmcnt<0>();  // nothing is under way into LDS when the workgroup ends
     if (bad && a.bt.status && tid == 0) atomicOr(&a.bt.status[t.b], PAGE_SEQ_BAD_PAGE);
     l = half_sum(l);
     if (r >= rows) return;
@@ -936,6 +957,8 @@ __global__ __launch_bounds__(PF_WAVES * 64, 2) void paged_prompt_kernel(PagedAtt
 // ---------------------------------------------------------------------------
 // launch plan
 // ---------------------------------------------------------------------------
+constexpr int PA_CUS = 256;  // compute units of the part
+
 struct Plan {
     bool prompt;
     int nt, tiles, splits, per;  // 16-row column tiles of a workgroup, tiles of a (sequence, kv head), splits, blocks each
@@ -945,7 +968,13 @@ Plan plan_of(const PagedAttnArgs& a) {
     const int group = a.n_heads / a.pool.n_kv;
     const long long rows = (long long)a.bt.max_rows * group;
     Plan p{};
-    p.prompt = rows > 32;
+    // Rows up to which a second or fourth pass over the cache by 32-row tiles is quicker than 128-row tiles with their
+    // barriers.  Measured: fp16, 8 x 24 tokens of 4 heads over 4096 67 us in tiles of 32, 49 in tiles of 128; 1 x 32 25
+    // and 31; 32 x 16 over 1000 47 and 39; head_dim 64, 16 x 100 of one head over 1000 28 and 37; f32 over
+    // INT8, 8 x 24 over 4096 81 and 94.
+    const long long pairs = (long long)a.bt.nseq * a.pool.n_kv;
+    const int few = a.pool.hd == 64 || a.pool.fmt == KV_INT8 || pairs <= 16 ? 128 : pairs <= 128 ? 64 : 32;
+    p.prompt = rows > few;
     p.nt = rows <= 16 ? 1 : 2;
     const int tile_rows = p.prompt ? PF_ROWS : 16 * p.nt;
     p.tiles = (int)((rows + tile_rows - 1) / tile_rows);
@@ -953,11 +982,28 @@ Plan plan_of(const PagedAttnArgs& a) {
     const int all = (a.bt.max_kv + 31) / 32;
     const int span = (tile_rows + group - 1) / group + 1;
     const int n = a.window && !a.prefix ? (int)std::min<long long>(all, ((long long)a.window + span) / 32 + 2) : all;
-    // two workgroups per compute unit; a wave (or a workgroup that shares its blocks) gets at least two blocks or steps
     const long long base = (long long)a.bt.nseq * a.pool.n_kv * p.tiles;
-    const int want = (int)std::max<long long>(1, (512 + base - 1) / base);
-    const int unit = p.prompt ? 2 : DC_WAVES;
-    p.splits = std::max(1, std::min(want, n / (2 * unit)));
+    const int unit = p.prompt ? 2 : dc_waves(a.pool.fmt);  // blocks of a step (prompt) or of a round of the waves
+    if (p.prompt) {
+        // Fewer steps for a workgroup against more partial results and a second launch.  Measured at head_dim 128, fp16: 1.5 us
+        // a step with one workgroup on a compute unit, 2 us each with two; 3 us to start, 4 us and 3.5 TB/s to join.
+        const double step = (0.5 + a.pool.hd / 128.0) * (a.act == ACT_F32 ? 1.6 : 1.0) * (a.pool.fmt == KV_INT8 ? 1.3 : 1.0);
+        double best = 0;
+        p.splits = 1;
+        for (int k = 1; k <= std::min(32, std::max(1, n / 4)); k++) {
+            const double per_cu = std::ceil((double)(base * k) / PA_CUS);
+            const double steps = std::ceil((n + 1) / 2 / (double)k);
+            double us = (3 + steps * step) * (per_cu <= 1 ? 1.0 : per_cu * 0.67);
+            if (k > 1) us += 4 + (double)a.bt.rows * a.n_heads * k * (a.pool.hd + 2) * 8 / 3.5e6;
+            if (k == 1 || us < 0.95 * best) {
+                best = us;
+                p.splits = k;
+            }
+        }
+    } else {
+        // a workgroup per compute unit, a block for each wave (64 splits at most: a lane each when they are joined)
+        p.splits = (int)std::min<long long>(std::min(64, std::max(1, n / unit)), std::max<long long>(1, (PA_CUS + base - 1) / base));
+    }
     p.per = (n + p.splits - 1) / p.splits;
     p.per = (p.per + unit - 1) / unit * unit;
     p.splits = std::max(1, (n + p.per - 1) / p.per);
@@ -971,18 +1017,15 @@ int launch_hd(const PagedAttnArgs& a, hipStream_t stream) {
     const long long blocks = (long long)a.bt.nseq * a.pool.n_kv * p.tiles * p.splits;
     if (blocks > 0x7fffffffLL / 256) return note_error(hipErrorInvalidConfiguration);
     const dim3 grid((unsigned)blocks);
-    auto go = [&](auto kernel, unsigned lds) {
-        hipLaunchKernelGGL(kernel, grid, dim3(256), lds, stream, a, group, p.tiles, p.splits, p.per);
-    };
-    const unsigned lds = 8 * PAGE_BLK * HD * (KVF == KV_INT8 ? 1 : 2);
-    if (p.prompt && a.slopes) go(paged_prompt_kernel<T, KVF, HD, 2>, lds);
-    else if (p.prompt && a.softcap > 0.f) go(paged_prompt_kernel<T, KVF, HD, 1>, lds);
-    else if (p.prompt) go(paged_prompt_kernel<T, KVF, HD, 0>, lds);
-    else if (p.nt == 1) go(paged_decode_kernel<T, KVF, HD, 1>, 0);
-    else go(paged_decode_kernel<T, KVF, HD, 2>, 0);
+    auto go = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, dim3(p.prompt ? 256 : dc_waves(KVF) * 64), 0, stream, a, group, p.tiles, p.splits, p.per); };
+    if (p.prompt && a.slopes) go(paged_prompt_kernel<T, KVF, HD, 2>);
+    else if (p.prompt && a.softcap > 0.f) go(paged_prompt_kernel<T, KVF, HD, 1>);
+    else if (p.prompt) go(paged_prompt_kernel<T, KVF, HD, 0>);
+    else if (p.nt == 1) go(paged_decode_kernel<T, KVF, HD, 1>);
+    else go(paged_decode_kernel<T, KVF, HD, 2>);
     if (p.splits > 1) {
-        const long long n = (long long)a.bt.max_rows * a.n_heads * (HD / 4);
-        hipLaunchKernelGGL((paged_merge_kernel<T, HD>), dim3((unsigned)((n + 255) / 256), a.bt.nseq), dim3(256), 0, stream, a, p.splits);
+        const long long n = (long long)a.bt.max_rows * a.n_heads;
+        hipLaunchKernelGGL((paged_merge_kernel<T, HD>), dim3((unsigned)((n + 3) / 4), a.bt.nseq), dim3(256), 0, stream, a, p.splits);
     }
     return note_error(hipGetLastError());
 }
