@@ -478,7 +478,7 @@ typedef struct {
     int64_t history_ld;
     const int32_t *history_len; /* [nseq] */
     const int32_t *prompt_len;  /* [nseq], NULL: 0 */
-    const float *penalties;     /* [nseq][3] repetition (> 0), presence, frequency; NULL: none */
+    const float *penalties;     /* [nseq][3] repetition (> 0, finite), presence, frequency; NULL: none */
     const uint32_t *draft;      /* [nseq][draft_ld >= rows_per_seq - 1], NULL: none */
     int64_t draft_ld;
     const int32_t *bias_off;    /* [nseq + 1] into the next two, NULL: none */
