@@ -17,6 +17,7 @@ CPU fallback: a missing or unloadable library raises immediately.
 import atexit
 import collections
 import ctypes as C
+import functools
 import os
 import weakref
 from dataclasses import dataclass, field
@@ -384,7 +385,7 @@ def _on(device, name, t, dtype, dim, contiguous=True):
     """Data pointer of a device tensor (None: NULL) after its checks."""
     if t is None:
         return None
-    if t.device.type != "cuda" or t.device.index != device:
+    if not t.is_cuda or t.get_device() != device:
         raise ConfigError(f"{name} must be on cuda:{device}, not {t.device}")
     if t.dtype != dtype:
         raise UnsupportedError(f"{name} must be {dtype}, not {t.dtype}")
@@ -397,8 +398,21 @@ def _on(device, name, t, dtype, dim, contiguous=True):
 
 def _stream(device):
     """The current torch stream as the C ABI takes it (the default stream has a value of its own there)."""
+    return _raw_stream()(device) or DEFAULT_STREAM
+
+
+@functools.lru_cache(None)
+def _raw_stream():
+    """How to ask torch for the current stream's handle of a device."""
     import torch
-    return torch.cuda.current_stream(device).cuda_stream or DEFAULT_STREAM
+    return getattr(torch._C, "_cuda_getCurrentRawStream", None) or \
+        (lambda device: torch.cuda.current_stream(device).cuda_stream)
+
+
+@functools.lru_cache(None)
+def _act_formats():
+    import torch
+    return {torch.float32: A_F32, torch.float16: A_F16, torch.bfloat16: A_BF16}
 
 
 class PagePool:
@@ -807,13 +821,12 @@ class HipModel:
     # ------------------------------------------------------------------
     def _act(self, name, t, rows, heads, hd):
         """(activation format, row stride) of a [rows, heads, head_dim] tensor whose rows may be apart."""
-        import torch
-        act = {torch.float32: A_F32, torch.float16: A_F16, torch.bfloat16: A_BF16}.get(t.dtype)
+        act = _act_formats().get(t.dtype)
         if act is None:
             raise UnsupportedError(f"{name} must be float32, float16 or bfloat16, not {t.dtype}")
-        if t.device.type != "cuda" or t.device.index != self.device:
+        if not t.is_cuda or t.get_device() != self.device:
             raise ConfigError(f"{name} must be on cuda:{self.device}, not {t.device}")
-        if t.dim() != 3 or t.shape[0] != rows or t.shape[1] != heads or t.shape[2] != hd:
+        if t.shape != (rows, heads, hd):
             raise ShapeError(f"{name} must be {(rows, heads, hd)}, not {tuple(t.shape)}")
         sr, sh, sd = t.stride()
         if (hd > 1 and sd != 1) or (heads > 1 and sh != hd):
@@ -841,8 +854,9 @@ class HipModel:
             heads = q.shape[1]
             q_act, q_ld = self._act("q", q, n, heads, hd)
             if out is None:
-                out = torch.empty((n, heads, hd), dtype=q.dtype, device=q.device)
-            o_act, o_ld = self._act("out", out, n, heads, hd)
+                out, o_act, o_ld = q.new_empty((n, heads, hd)), q_act, heads * hd
+            else:
+                o_act, o_ld = self._act("out", out, n, heads, hd)
             if q_act != act or o_act != act:
                 raise UnsupportedError("q, k, v and out must have one type")
         if v_act != act:
@@ -866,10 +880,11 @@ class HipModel:
         n, hd, heads = batch.rows, pool.head_dim, q.shape[1] if q.dim() == 3 else 0
         act, q_ld = self._act("q", q, n, heads, hd)
         if out is None:
-            out = torch.empty((n, heads, hd), dtype=q.dtype, device=q.device)
-        o_act, o_ld = self._act("out", out, n, heads, hd)
-        if o_act != act:
-            raise UnsupportedError("q and out must have one type")
+            out, o_ld = q.new_empty((n, heads, hd)), heads * hd
+        else:
+            o_act, o_ld = self._act("out", out, n, heads, hd)
+            if o_act != act:
+                raise UnsupportedError("q and out must have one type")
         sl = _on(self.device, "slopes", slopes, torch.float32, 1)
         pre = _on(self.device, "prefix", prefix, torch.int32, 1)
         if (slopes is not None and slopes.shape[0] != heads) or (prefix is not None and prefix.shape[0] != batch._c.nseq):
@@ -904,16 +919,16 @@ class HipModel:
             raise ShapeError(f"logits {tuple(logits.shape)} are not rows of {rows_per_seq} for each sequence")
         rows, V = logits.shape
         n, dev, i32, f32 = rows // rows_per_seq, self.device, torch.int32, torch.float32
-        if out is None:
-            out = torch.empty((rows, V), dtype=f32, device=logits.device)
         for name, t in (("logits", logits), ("out", out)):
             _on(dev, name, t, f32, 2, contiguous=False)
-            if tuple(t.shape) != (rows, V) or (V > 1 and t.stride(1) != 1):
+            if t is not None and (t.shape != (rows, V) or (V > 1 and t.stride(1) != 1)):
                 raise UnsupportedError(f"{name} must be {(rows, V)} with contiguous rows")
+        if out is None:
+            out = logits.new_empty((rows, V))
         for name, t, shape in (("history_len", history_len, (n,)), ("prompt_len", prompt_len, (n,)),
                                ("penalties", penalties, (n, 3)), ("bias_off", bias_off, (n + 1,)),
                                ("mask_of_row", mask_of_row, (rows,))):
-            if t is not None and tuple(t.shape) != shape:
+            if t is not None and t.shape != shape:
                 raise ShapeError(f"{name} must be {shape}, not {tuple(t.shape)}")
         if (history is not None and history.shape[0] != n) or (draft is not None and draft.shape[0] != n):
             raise ShapeError(f"history and draft must have a row for each of {n} sequences")
