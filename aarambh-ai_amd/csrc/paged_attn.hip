@@ -117,6 +117,23 @@ __device__ __forceinline__ bool tile_info(const PagedAttnArgs& a, int b, int kvh
     return true;
 }
 
+// Tokens base .. base + n - 1 as bits: those from low to high, and those before pre.
+__device__ __forceinline__ uint32_t seen_bits(int base, int low, int high, int pre, int n) {
+    auto ones = [](int k) { return k >= 32 ? 0xFFFFFFFFu : (1u << k) - 1u; };
+    auto upto = [&](int t) { return ones(min(max(t - base, 0), n)); };
+    return (upto(high + 1) & ~upto(low)) | upto(pre);
+}
+// 16-bit masks of eight tokens (bits of b)
+__device__ __forceinline__ u32x4_t keep_words(uint32_t b) {
+    u32x4_t k;
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        const uint32_t lo = (uint32_t)((int32_t)(b << (31 - 2 * i)) >> 31), hi = (uint32_t)((int32_t)(b << (30 - 2 * i)) >> 31);
+        k[i] = (lo & 0xFFFFu) | (hi & 0xFFFF0000u);
+    }
+    return k;
+}
+
 __device__ __forceinline__ int tile_block(const TileInfo& t, int k) { return k < t.pre_blk ? k : t.lo_blk + (k - t.pre_blk); }
 
 __device__ __forceinline__ int head_of(const PagedAttnArgs& a, int kvh, int m, int group) {
@@ -329,21 +346,20 @@ __global__ __launch_bounds__(dc_waves(KVF) * 64) void paged_decode_kernel(PagedA
             }
             float c = qs[nt] * PA_LOG2E;
             if (!plain) {
+                const float at = slope[nt] * (float)(t0 + 8 * lg - pos[nt]);
+                if (a.softcap > 0.f) {
 #pragma unroll
-                for (int i = 0; i < 8; i++) {
-                    x[i] *= qs[nt];
-                    if (a.softcap > 0.f) x[i] = a.softcap * tanh_f32<F32>(x[i] * inv_cap);
-                    x[i] = x[i] * PA_LOG2E + slope[nt] * (float)(t0 + 8 * lg + i - pos[nt]);
+                    for (int i = 0; i < 8; i++) x[i] = a.softcap * tanh_f32<F32>(x[i] * qs[nt] * inv_cap);
+                    c = PA_LOG2E;
                 }
+#pragma unroll
+                for (int i = 0; i < 8; i++) x[i] = fmaf(x[i], c, fmaf(slope[nt], (float)i, at));
                 c = 1.f;
             }
             if (!whole) {
+                const uint32_t seen = absent ? 0u : seen_bits(t0 + 8 * lg, a.window ? max(0, pos[nt] - a.window + 1) : 0, pos[nt], t.pre, 8);
 #pragma unroll
-                for (int i = 0; i < 8; i++) {
-                    const int tok = t0 + 8 * lg + i;
-                    const bool seen = !absent && ((tok <= pos[nt] && (a.window == 0 || pos[nt] - tok < a.window)) || tok < t.pre);
-                    x[i] = seen ? x[i] : -INFINITY;
-                }
+                for (int i = 0; i < 8; i++) x[i] = (seen >> i) & 1u ? x[i] : -INFINITY;
             }
             float mx = x[0];
 #pragma unroll
@@ -375,18 +391,7 @@ __global__ __launch_bounds__(dc_waves(KVF) * 64) void paged_decode_kernel(PagedA
         // tokens that no row sees may hold anything, also NaN: their V is taken as zero
         if constexpr (!I8) {
             if (!whole) {
-                u32x4_t keep;
-#pragma unroll
-                for (int i = 0; i < 4; i++) {
-                    uint32_t w = 0;
-#pragma unroll
-                    for (int e = 0; e < 2; e++) {
-                        const int tok = t0 + 8 * lg + 2 * i + e;
-                        const bool any = (tok <= t.p_hi && tok >= t.low) || tok < t.pre;
-                        w |= any && !absent ? 0xFFFFu << (16 * e) : 0u;
-                    }
-                    keep[i] = w;
-                }
+                const u32x4_t keep = keep_words(absent ? 0u : seen_bits(t0 + 8 * lg, t.low, t.p_hi, t.pre, 8));
 #pragma unroll
                 for (int i = 0; i < KL; i++) vr[i] &= keep;
             }
@@ -523,6 +528,18 @@ __device__ __forceinline__ float half_sum(float x) {
     return __uint_as_float(b[0]) + __uint_as_float(b[1]);
 }
 
+// Piece i (of 4) of 1 KiB steps from a buffer offset to LDS: the instruction's offset counts for both sides, so four
+// pieces share M0 and the scalar offset.
+__device__ __forceinline__ void lds_piece(__amdgpu_buffer_rsrc_t r, const void* lds_dst, int voff, int soff, int i) {
+    const unsigned base = __builtin_amdgcn_readfirstlane((unsigned)(uintptr_t)lds_dst);
+    switch (i) {
+        case 0: asm volatile("s_nop 0\n\tbuffer_load_dwordx4 %0, %1, %2 offen lds" ::"v"(voff), "s"(r), "s"(soff), "{m0}"(base) : "memory"); break;
+        case 1: asm volatile("s_nop 0\n\tbuffer_load_dwordx4 %0, %1, %2 offen offset:1024 lds" ::"v"(voff), "s"(r), "s"(soff), "{m0}"(base) : "memory"); break;
+        case 2: asm volatile("s_nop 0\n\tbuffer_load_dwordx4 %0, %1, %2 offen offset:2048 lds" ::"v"(voff), "s"(r), "s"(soff), "{m0}"(base) : "memory"); break;
+        default: asm volatile("s_nop 0\n\tbuffer_load_dwordx4 %0, %1, %2 offen offset:3072 lds" ::"v"(voff), "s"(r), "s"(soff), "{m0}"(base) : "memory"); break;
+    }
+}
+
 constexpr int PF_WAVES = 4, PF_ROWS = 32 * PF_WAVES;
 
 // MODE 0: scores as they are, 1: capped, 2: a slope per head (capped or not)
@@ -620,7 +637,7 @@ __global__ __launch_bounds__(PF_WAVES * 64, 2) void paged_prompt_kernel(PagedAtt
 #pragma unroll
         for (int j = 0; j < 2; j++) {
             s.blk[j] = tile_block(t, min(k + j, k1 - 1));
-            s.page[j] = table[s.blk[j] >> shift];
+            s.page[j] = *(const int32_t*)((const char*)table + ((uint32_t)(s.blk[j] >> shift) << 2));
         }
         return s;
     };
@@ -653,7 +670,7 @@ __global__ __launch_bounds__(PF_WAVES * 64, 2) void paged_prompt_kernel(PagedAtt
                     pf_lds + buf * (4 * BLK) + (2 * my_v + my_j) * BLK};
     };
     auto piece = [&](const Load& ld, int i) __attribute__((always_inline)) {
-        lds_dma16(coh_rsrc((const void*)(((uint64_t)ld.hi << 32) | ld.lo)), ld.dst + i * 1024, my_src, i * 1024);
+        lds_piece(coh_rsrc((const void*)(((uint64_t)ld.hi << 32) | ld.lo)), ld.dst + (i & ~3) * 1024, my_src, (i & ~3) * 1024, i & 3);
     };
     auto pieces = [&](const Load& ld) __attribute__((always_inline)) {
 #pragma unroll
@@ -764,11 +781,7 @@ __global__ __launch_bounds__(PF_WAVES * 64, 2) void paged_prompt_kernel(PagedAtt
         if constexpr (MASK) {
 #pragma unroll
             for (int j = 0; j < 2; j++) {
-                // visible tokens of the block as bits: low .. pos, and those of the prefix
-                const int base = t0[j] + 8 * hk, low = a.window ? pos - a.window + 1 : 0;
-                const int hi_n = min(max(pos + 1 - base, 0), 32), lo_n = min(max(low - base, 0), 32), pre_n = min(max(t.pre - base, 0), 32);
-                auto ones = [](int n) { return n >= 32 ? 0xFFFFFFFFu : (1u << n) - 1u; };
-                const uint32_t seen = w.skip[j] ? 0u : (ones(hi_n) & ~ones(lo_n)) | ones(pre_n);
+                const uint32_t seen = w.skip[j] ? 0u : seen_bits(t0[j] + 8 * hk, a.window ? max(0, pos - a.window + 1) : 0, pos, t.pre, 32);
 #pragma unroll
                 for (int i = 0; i < 16; i++) s[j][i] = (seen >> (16 * (i >> 3) + (i & 7))) & 1u ? s[j][i] : -INFINITY;
             }
@@ -836,18 +849,7 @@ __global__ __launch_bounds__(PF_WAVES * 64, 2) void paged_prompt_kernel(PagedAtt
                 u32x4_t keep;
                 if constexpr (MASK && !I8) {
                     // tokens that no row of this wave sees may hold anything, also NaN
-                    const int base = t0[j] + 16 * g + 8 * hk;
-#pragma unroll
-                    for (int i = 0; i < 4; i++) {
-                        uint32_t kw = 0;
-#pragma unroll
-                        for (int e = 0; e < 2; e++) {
-                            const int tk = base + 2 * i + e;
-                            const bool any = !w.skip[j] & (((tk <= w_hi) & (tk >= wlow)) | (tk < t.pre));
-                            kw |= any ? 0xFFFFu << (16 * e) : 0u;
-                        }
-                        keep[i] = kw;
-                    }
+                    keep = keep_words(w.skip[j] ? 0u : seen_bits(t0[j] + 16 * g + 8 * hk, wlow, w_hi, t.pre, 8));
                 }
 #pragma unroll
                 for (int d = 0; d < DT; d++) {
