@@ -134,6 +134,16 @@ __device__ __forceinline__ u32x4_t keep_words(uint32_t b) {
     return k;
 }
 
+// Workgroup -> pair of sequence and kv head (fastest), tile of its rows, split of its keys.  Workgroups go to the
+// eight dies in turn, so tiles of a pair, which read the same blocks, share a die's cache when there are 8 n pairs.
+struct Place {
+    int pair, tile, split;
+};
+__device__ __forceinline__ Place place_of(const PagedAttnArgs& a, int tiles) {
+    const int pairs = a.bt.nseq * a.pool.n_kv, rest = blockIdx.x / pairs;
+    return {(int)blockIdx.x - rest * pairs, rest % tiles, rest / tiles};
+}
+
 __device__ __forceinline__ int tile_block(const TileInfo& t, int k) { return k < t.pre_blk ? k : t.lo_blk + (k - t.pre_blk); }
 
 __device__ __forceinline__ int head_of(const PagedAttnArgs& a, int kvh, int m, int group) {
@@ -157,7 +167,7 @@ __device__ __forceinline__ float2_t* part_ml(const PagedAttnArgs& a, int splits,
 // well with four (64 x 1 over 4096 6.3 TB/s either way) and have less to join.
 constexpr int dc_waves(int kvf) { return kvf == KV_INT8 ? 8 : 4; }
 
-template <typename T, int KVF, int HD, int NT>
+template <typename T, int KVF, int HD, int NT, bool ONCE>
 __global__ __launch_bounds__(dc_waves(KVF) * 64) void paged_decode_kernel(PagedAttnArgs a, int group, int tiles, int splits, int per) {
     typedef typename Mat<KVF>::frag frag;
     typedef typename Mat<KVF>::elem elem;
@@ -171,14 +181,10 @@ __global__ __launch_bounds__(dc_waves(KVF) * 64) void paged_decode_kernel(PagedA
     __shared__ float s_o[DC_WAVES][16 * LDO];
     __shared__ float2_t s_ml[DC_WAVES][16];
     const int tid = threadIdx.x, lane = tid & 63, wid = __builtin_amdgcn_readfirstlane(tid >> 6), lr = lane & 15, lg = lane >> 4;
-    // workgroup -> (pair of sequence and kv head, tile, split), pairs fastest
-    int id = blockIdx.x;
-    const int pairs = a.bt.nseq * a.pool.n_kv;
-    const int pair = id % pairs;
-    id /= pairs;
-    const int tile = id % tiles, split = id / tiles;
+    const Place at = place_of(a, tiles);
+    const int split = at.split;
     TileInfo t;
-    if (!tile_info(a, pair / a.pool.n_kv, pair % a.pool.n_kv, tile, 16 * NT, group, &t)) return;
+    if (!tile_info(a, at.pair / a.pool.n_kv, at.pair % a.pool.n_kv, at.tile, 16 * NT, group, &t)) return;
     const int k0 = split * per, k1 = min(k0 + per, t.n);
     const int rows = t.s.rows * group, pos0 = t.s.kv_len - t.s.rows;
 
@@ -262,16 +268,20 @@ __global__ __launch_bounds__(dc_waves(KVF) * 64) void paged_decode_kernel(PagedA
         const int p = page >= 0 && page < a.pool.n_pages ? page : 0;
         off = ((((size_t)p * a.pool.n_kv + t.kvh) << shift) + (blk & ((1 << shift) - 1))) * PAGE_BLK;
     };
-    auto load_k = [&]() __attribute__((always_inline)) {
-        const char* p = (const char*)a.pool.k + off * (BLK / PAGE_BLK) + lane * 16;
+    // ONCE: a block that no other workgroup reads does not stay in the caches
+    auto load_block = [&](u32x4_t(&r)[KL], const char* p) __attribute__((always_inline)) {
 #pragma unroll
-        for (int i = 0; i < KL; i++) kr[i] = __builtin_nontemporal_load((const u32x4_t*)(p + i * 1024));
+        for (int i = 0; i < KL; i++) {
+            if constexpr (ONCE) r[i] = __builtin_nontemporal_load((const u32x4_t*)(p + i * 1024));
+            else r[i] = *(const u32x4_t*)(p + i * 1024);
+        }
+    };
+    auto load_k = [&]() __attribute__((always_inline)) {
+        load_block(kr, (const char*)a.pool.k + off * (BLK / PAGE_BLK) + lane * 16);
         if constexpr (I8) ksc = *(const u32x4_t*)(a.pool.ks + off + 8 * lg);
     };
     auto load_v = [&]() __attribute__((always_inline)) {
-        const char* p = (const char*)a.pool.v + off * (BLK / PAGE_BLK) + (I8 ? lane : lr * 4 + lg) * 16;
-#pragma unroll
-        for (int i = 0; i < KL; i++) vr[i] = __builtin_nontemporal_load((const u32x4_t*)(p + i * 1024));
+        load_block(vr, (const char*)a.pool.v + off * (BLK / PAGE_BLK) + (I8 ? lane : lr * 4 + lg) * 16);
         if constexpr (I8) vsc = *(const u32x4_t*)(a.pool.vs + off + 8 * lg);
     };
     auto sc_at = [](u32x4_t s, int i) __attribute__((always_inline)) {
@@ -346,14 +356,14 @@ __global__ __launch_bounds__(dc_waves(KVF) * 64) void paged_decode_kernel(PagedA
             }
             float c = qs[nt] * PA_LOG2E;
             if (!plain) {
-                const float at = slope[nt] * (float)(t0 + 8 * lg - pos[nt]);
+                const float from = slope[nt] * (float)(t0 + 8 * lg - pos[nt]);
                 if (a.softcap > 0.f) {
 #pragma unroll
                     for (int i = 0; i < 8; i++) x[i] = a.softcap * tanh_f32<F32>(x[i] * qs[nt] * inv_cap);
                     c = PA_LOG2E;
                 }
 #pragma unroll
-                for (int i = 0; i < 8; i++) x[i] = fmaf(x[i], c, fmaf(slope[nt], (float)i, at));
+                for (int i = 0; i < 8; i++) x[i] = fmaf(x[i], c, fmaf(slope[nt], (float)i, from));
                 c = 1.f;
             }
             if (!whole) {
@@ -554,13 +564,10 @@ __global__ __launch_bounds__(PF_WAVES * 64, 2) void paged_prompt_kernel(PagedAtt
     constexpr int KIB = BLK / 1024;  // wave loads of a block of K (or V)
     __shared__ __attribute__((aligned(1024))) char pf_lds[8 * BLK];  // [2 stages][K: 2 blocks | V: 2 blocks]
     const int tid = threadIdx.x, lane = tid & 63, wid = __builtin_amdgcn_readfirstlane(tid >> 6), hk = lane >> 5, m = lane & 31;
-    int id = blockIdx.x;
-    const int pairs = a.bt.nseq * a.pool.n_kv;
-    const int pair = id % pairs;
-    id /= pairs;
-    const int tile = tiles - 1 - id % tiles, split = id / tiles;  // the longest rows first
-    TileInfo t;
-    if (!tile_info(a, pair / a.pool.n_kv, pair % a.pool.n_kv, tile, PF_ROWS, group, &t)) return;
+    const Place place = place_of(a, tiles);
+    const int split = place.split;
+    TileInfo t;  // the longest rows first
+    if (!tile_info(a, place.pair / a.pool.n_kv, place.pair % a.pool.n_kv, tiles - 1 - place.tile, PF_ROWS, group, &t)) return;
     const int k0 = split * per, k1 = min(k0 + per, t.n);
     const int rows = t.s.rows * group, pos0 = t.s.kv_len - t.s.rows;
 
@@ -970,14 +977,22 @@ Plan plan_of(const PagedAttnArgs& a) {
     const int group = a.n_heads / a.pool.n_kv;
     const long long rows = (long long)a.bt.max_rows * group;
     Plan p{};
-    // Rows up to which a second or fourth pass over the cache by 32-row tiles is quicker than 128-row tiles with their
-    // barriers.  Measured: fp16, 8 x 24 tokens of 4 heads over 4096 67 us in tiles of 32, 49 in tiles of 128; 1 x 32 25
-    // and 31; 32 x 16 over 1000 47 and 39; head_dim 64, 16 x 100 of one head over 1000 28 and 37; f32 over
-    // INT8, 8 x 24 over 4096 81 and 94.
+    // Tiles of 16 or 32 rows stream the cache through the registers, each tile by itself (from the die's cache after the first);
+    // tiles of 128 rows share it through LDS and take longer to start.  The former are quicker for one tile of 32 and
+    // while there is little to do in all: few tiles, few blocks for them.  Measured, in us (tiles of 16 or 32 / of
+    // 128): fp16, head_dim 128, 4 heads a kv head, sequences x rows over tokens: 1 x 256 over 256 12 / 21, 1 x 160 over 2000
+    // 26 / 32, over 8000 83 / 51, 8 x 16 over 4096 41 / 41, 8 x 24 62 / 47, 32 x 12 253 / 120, 4 x 128 over 0 14 / 11;
+    // head_dim 64, 12 heads: 16 x 64 over 1000 19 / 25, 16 x 128 29 / 30, over 4096 98 / 81; f32
+    // over INT8 (whose codes 128-row tiles convert in every wave): 1 x 64 27 / 49, 8 x 40 105 / 143, 8 x 64 over 8000 157 / 189.
     const long long pairs = (long long)a.bt.nseq * a.pool.n_kv;
-    const int few = a.pool.hd == 64 || a.pool.fmt == KV_INT8 || pairs <= 16 ? 128 : pairs <= 128 ? 64 : 32;
-    p.prompt = rows > few;
-    p.nt = rows <= 16 ? 1 : 2;
+    const int seen = a.window && !a.prefix ? (int)std::min<long long>(a.bt.max_kv, (long long)a.window + a.bt.max_rows) : a.bt.max_kv;
+    const long long f = (a.pool.hd == 64 ? 2 : 1) * (a.pool.fmt == KV_INT8 ? 8 : 1);
+    p.prompt = rows > 32 && (rows * pairs > 8192 * f || rows * pairs * ((seen + 31) / 32) > 540000 * f);
+    // One 16-row tile a workgroup where that leaves every workgroup a compute unit of its own or wastes less than 32-row tiles,
+    // which read the cache half as often (8 rows x 4 heads, 4096 tokens: 1 sequence 13 us and 16, 32 sequences 146 and 91;
+    // 33 rows over 1000, 16 x 12 heads of 64: 14.5 and 18.5).
+    const long long tiles16 = (rows + 15) / 16;
+    p.nt = tiles16 == 1 || tiles16 == 3 || pairs * tiles16 <= (a.pool.hd == 64 && tiles16 > 2 ? 2 : 1) * PA_CUS ? 1 : 2;
     const int tile_rows = p.prompt ? PF_ROWS : 16 * p.nt;
     p.tiles = (int)((rows + tile_rows - 1) / tile_rows);
     // blocks that a tile can visit
@@ -1003,8 +1018,10 @@ Plan plan_of(const PagedAttnArgs& a) {
             }
         }
     } else {
-        // a workgroup per compute unit, a block for each wave (64 splits at most: a lane each when they are joined)
-        p.splits = (int)std::min<long long>(std::min(64, std::max(1, n / unit)), std::max<long long>(1, (PA_CUS + base - 1) / base));
+        // A block for each wave, and as many workgroups as compute units (twice as many at head_dim 64: 10 x 12 heads over
+        // 4096 27 us and 31; at 128 32 x 4 rows over INT8 60 and 51) but not more, so that they end together (20 x 8 kv heads:
+        // 160 workgroups 58 us, 320 68).  64 splits at most: a lane each when they are joined.
+        p.splits = (int)std::min<long long>(std::min(64, std::max(1, n / unit)), std::max<long long>(1, (a.pool.hd == 64 ? 2 : 1) * PA_CUS / base));
     }
     p.per = (n + p.splits - 1) / p.splits;
     p.per = (p.per + unit - 1) / unit * unit;
@@ -1023,8 +1040,10 @@ int launch_hd(const PagedAttnArgs& a, hipStream_t stream) {
     if (p.prompt && a.slopes) go(paged_prompt_kernel<T, KVF, HD, 2>);
     else if (p.prompt && a.softcap > 0.f) go(paged_prompt_kernel<T, KVF, HD, 1>);
     else if (p.prompt) go(paged_prompt_kernel<T, KVF, HD, 0>);
-    else if (p.nt == 1) go(paged_decode_kernel<T, KVF, HD, 1>);
-    else go(paged_decode_kernel<T, KVF, HD, 2>);
+    else if (p.nt == 1 && p.tiles == 1) go(paged_decode_kernel<T, KVF, HD, 1, true>);
+    else if (p.nt == 1) go(paged_decode_kernel<T, KVF, HD, 1, false>);
+    else if (p.tiles == 1) go(paged_decode_kernel<T, KVF, HD, 2, true>);
+    else go(paged_decode_kernel<T, KVF, HD, 2, false>);
     if (p.splits > 1) {
         const long long n = (long long)a.bt.max_rows * a.n_heads;
         hipLaunchKernelGGL((paged_merge_kernel<T, HD>), dim3((unsigned)((n + 3) / 4), a.bt.nseq), dim3(256), 0, stream, a, p.splits);
