@@ -1057,7 +1057,7 @@ int launch_hd(const PagedAttnArgs& a, hipStream_t stream) {
     const Plan p = plan_of(a);
     const int group = a.n_heads / a.pool.n_kv;
     const long long blocks = (long long)a.bt.nseq * a.pool.n_kv * p.tiles * p.splits;
-    if (blocks > 0x7fffffffLL / 256) return note_error(hipErrorInvalidConfiguration);
+    if (blocks > 0x7fffffffLL / 256) return note_error(hipErrorInvalidConfiguration);  // (the entry refuses such calls)
     const dim3 grid((unsigned)blocks);
     auto go = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, dim3(p.prompt ? 256 : dc_waves(KVF) * 64), 0, stream, a, group, p.tiles, p.splits, p.per); };
     if (p.prompt && a.slopes) go(paged_prompt_kernel<T, KVF, HD, 2>);

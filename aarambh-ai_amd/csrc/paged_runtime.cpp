@@ -134,6 +134,9 @@ int attn_args(aarh_ctx* c, const aarh_page_pool* pool, const aarh_page_batch* ba
         return r;
     if (args->n_heads <= 0 || args->n_heads > 65535 || args->n_heads % pool->n_kv_heads)
         return fail(c, AARH_ERR_SHAPE, "%d query heads over %d kv heads", args->n_heads, pool->n_kv_heads);
+    const int64_t rows = (int64_t)a->bt.max_rows * (args->n_heads / pool->n_kv_heads);
+    if (rows > (1 << 30) || (int64_t)batch->nseq * pool->n_kv_heads * (rows / 128 + 1) > (1 << 23))  // workgroups of a grid
+        return fail(c, AARH_ERR_SHAPE, "%d sequences of up to %d rows are too much for one call", batch->nseq, a->bt.max_rows);
     if (!shapes && (!std::isfinite(args->scale) || !(args->softcap >= 0.f) || !std::isfinite(args->softcap)))
         return fail(c, AARH_ERR_CONFIG, "scale must be finite, softcap finite and not negative");
     if (args->window < 0) return fail(c, AARH_ERR_CONFIG, "negative attention window %d", args->window);

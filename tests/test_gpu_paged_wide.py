@@ -174,6 +174,19 @@ def test_a_captured_decode_step(ctx):
         assert torch.equal(a.view(torch.int16), b.view(torch.int16))
 
 
+def test_grids_past_their_bound_are_refused(ctx):
+    pool = A.PagePool.allocate(1, 8, 64, 32)
+    n, rows = 60000, 2300
+    zeros = lambda *shape: torch.zeros(shape, dtype=torch.int32, device=DEV)  # noqa: E731
+    q = torch.ones((rows, 8, 64), dtype=torch.float16, device=DEV)
+    out = torch.full_like(q, 5.0)
+    with pytest.raises(A.ShapeError):
+        ctx.paged_attention(pool, A.PageBatch(zeros(n, 72), zeros(n), zeros(n + 1), rows=rows, max_rows=rows, max_kv=2300), q, out=out)
+    # as many sequences without rows, in a call made for one row each: nothing to do
+    ctx.paged_attention(pool, A.PageBatch(zeros(n, 1), zeros(n), zeros(n + 1), rows=rows, max_rows=1, max_kv=32), q, out=out)
+    assert torch.all(out == 5.0)
+
+
 @pytest.mark.parametrize("act,kv,hd,rows,lens", [("f16", "f16", 128, [300], [900]), ("bf16", "bf16", 64, [300, 280], [700, 900]),
                                                  ("f32", "f16", 128, [290], [1500])])
 def test_many_rows_over_a_few_splits(ctx, act, kv, hd, rows, lens):
