@@ -134,6 +134,48 @@ __device__ __forceinline__ u32x4_t keep_words(uint32_t b) {
     return k;
 }
 
+// Values that are not finite.  In a product they would also reach the rows that do not see their token (0 x inf), so where rows of
+// a tile see different tokens of a block such values are taken out of V and counted for the rows that do see them.
+template <int KVF>
+struct Odd {
+    static constexpr bool BF = KVF == KV_BF16;
+    static constexpr uint32_t INF = BF ? 0x7F80u : 0x7C00u, ONE = BF ? 0x3F80u : 0x3C00u, C64 = BF ? 0x4280u : 0x5400u, C4096 = BF ? 0x4580u : 0x6C00u;
+    typedef typename Mat<KVF>::frag frag;
+    typedef unsigned short u16x2_t __attribute__((ext_vector_type(2)));
+    // largest magnitude of both halves
+    static __device__ __forceinline__ uint32_t top(u32x4_t w, uint32_t t) {
+#pragma unroll
+        for (int i = 0; i < 4; i++)
+            t = __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(u16x2_t, w[i] & 0x7FFF7FFFu), __builtin_bit_cast(u16x2_t, t)));
+        return t;
+    }
+    static __device__ __forceinline__ bool any(uint32_t t) { return __any((t & 0xFFFFu) >= INF || t >> 16 >= INF); }
+    // marks to be counted: 1 for +inf, 64 for -inf, 4096 for NaN (a block has 32 tokens)
+    static __device__ __forceinline__ frag marks(u32x4_t w) {
+        auto mark = [](uint32_t h) {
+            const uint32_t m = h & 0x7FFFu;
+            return m < INF ? 0u : m > INF ? C4096 : h == INF ? ONE : C64;
+        };
+        u32x4_t r;
+#pragma unroll
+        for (int i = 0; i < 4; i++) r[i] = mark(w[i] & 0xFFFFu) | mark(w[i] >> 16) << 16;
+        return __builtin_bit_cast(frag, r);
+    }
+    static __device__ __forceinline__ u32x4_t finite(u32x4_t w) {
+#pragma unroll
+        for (int i = 0; i < 4; i++)
+            w[i] &= ((w[i] & 0x7FFFu) >= INF ? 0u : 0xFFFFu) | ((w[i] >> 16 & 0x7FFFu) >= INF ? 0u : 0xFFFF0000u);
+        return w;
+    }
+    // eight tokens' visibility as an operand
+    static __device__ __forceinline__ frag seen(uint32_t bits) { return __builtin_bit_cast(frag, keep_words(bits) & (ONE | ONE << 16)); }
+    // what the sum of the marks that a row sees adds to its result
+    static __device__ __forceinline__ float worth(float marks) {
+        const int n = (int)marks;
+        return (n & 63 ? INFINITY : 0.f) + (n >> 6 & 63 ? -INFINITY : 0.f) + (n >> 12 ? NAN : 0.f);
+    }
+};
+
 // Workgroup -> pair of sequence and kv head (fastest), tile of its rows, split of its keys.  Workgroups go to the
 // eight dies in turn, so tiles of a pair, which read the same blocks, share a die's cache when there are 8 n pairs.
 struct Place {
@@ -340,7 +382,7 @@ __global__ __launch_bounds__(dc_waves(KVF) * 64) void paged_decode_kernel(PagedA
             for (int i = 0; i < 8; i++) {
                 const int tok = t0 + 8 * lg + i;
                 const float v = sc_at(vsc, i);
-                top = fmaxf(top, tok < t.s.kv_len ? v : 0.f);
+                top = fmaxf(top, tok <= t.p_hi || tok < t.pre ? v : 0.f);
             }
             top = row16_max(top);
             vexp = top > 0x1p-20f ? (float)__builtin_amdgcn_frexp_expf(top) : -20.f;
@@ -404,6 +446,29 @@ __global__ __launch_bounds__(dc_waves(KVF) * 64) void paged_decode_kernel(PagedA
                 const u32x4_t keep = keep_words(absent ? 0u : seen_bits(t0 + 8 * lg, t.low, t.p_hi, t.pre, 8));
 #pragma unroll
                 for (int i = 0; i < KL; i++) vr[i] &= keep;
+                if (t.p_lo < t.p_hi && t0 + PAGE_BLK > t.pre) {
+                    uint32_t top = 0;
+#pragma unroll
+                    for (int i = 0; i < KL; i++) top = Odd<KVF>::top(vr[i], top);
+                    if (__builtin_expect(Odd<KVF>::any(top), 0)) {
+                        frag seen[NT];
+#pragma unroll
+                        for (int nt = 0; nt < NT; nt++)
+                            seen[nt] = Odd<KVF>::seen(absent ? 0u : seen_bits(t0 + 8 * lg, a.window ? max(0, pos[nt] - a.window + 1) : 0, pos[nt], t.pre, 8));
+#pragma unroll
+                        for (int d = 0; d < DT; d++) {
+                            const frag marks = Odd<KVF>::marks(vr[d]);
+                            vr[d] = Odd<KVF>::finite(vr[d]);
+#pragma unroll
+                            for (int nt = 0; nt < NT; nt++) {
+                                const float4_t c = mfma16<KVF>(marks, seen[nt], float4_t{0.f, 0.f, 0.f, 0.f});
+#pragma unroll
+                                for (int i = 0; i < 4; i++) o[nt][d][i] += Odd<KVF>::worth(c[i]);
+                            }
+                            __builtin_amdgcn_sched_barrier(0);  // (one at a time: few registers)
+                        }
+                    }
+                }
             }
         }
 #pragma unroll
@@ -787,7 +852,7 @@ __global__ __launch_bounds__(PF_WAVES * 64, 2) void paged_prompt_kernel(PagedAtt
                         s[j][8 * g + i] *= (float)ksc[i];
                         const float v = (float)vs[i];
                         vsc[j][8 * g + i] = v;
-                        top = fmaxf(top, !MASK || t0[j] + 16 * g + 8 * hk + i < t.s.kv_len ? v : 0.f);
+                        top = fmaxf(top, !MASK || t0[j] + 16 * g + 8 * hk + i < max(w_hi + 1, t.pre) ? v : 0.f);
                     }
                 }
             }
@@ -860,6 +925,30 @@ __global__ __launch_bounds__(PF_WAVES * 64, 2) void paged_prompt_kernel(PagedAtt
 #pragma unroll
                 for (int i = 0; i < 16; i++) s[j][i] = __builtin_amdgcn_exp2f(fmaf(s[j][i], c, -ref));
         }
+        auto v_at = [&](int j, int g, int d) __attribute__((always_inline)) { return *(const u32x4_t*)(vb + j * BLK + (v_lane ^ (g * 32)) + d * 2048); };
+        // tokens that no row of this wave sees may hold anything, also NaN
+        auto keep_of = [&](int j, int g) __attribute__((always_inline)) {
+            return keep_words(w.skip[j] ? 0u : seen_bits(t0[j] + 16 * g + 8 * hk, wlow, w_hi, t.pre, 8));
+        };
+        bool odd = false;
+        if constexpr (MASK && !I8) {
+            bool mixed = false;  // blocks of which the rows of this wave see different tokens
+#pragma unroll
+            for (int j = 0; j < 2; j++)
+                mixed |= !w.skip[j] && t0[j] + PAGE_BLK > t.pre && (t0[j] + PAGE_BLK - 1 > w_lo || (a.window && t0[j] <= w_hi - a.window));
+            if (mixed && w_lo < w_hi) {
+                uint32_t top = 0;
+#pragma unroll
+                for (int j = 0; j < 2; j++)
+#pragma unroll
+                    for (int g = 0; g < 2; g++) {
+                        const u32x4_t keep = keep_of(j, g);
+#pragma unroll
+                        for (int d = 0; d < DT; d++) top = Odd<KVF>::top(v_at(j, g, d) & keep, top);
+                    }
+                odd = Odd<KVF>::any(top);
+            }
+        }
 #pragma unroll
         for (int j = 0; j < 2; j++)
 #pragma unroll
@@ -877,10 +966,7 @@ __global__ __launch_bounds__(PF_WAVES * 64, 2) void paged_prompt_kernel(PagedAtt
                     if constexpr (F32) pl[i] = (elem)(p - (float)ph[i]);
                 }
                 u32x4_t keep;
-                if constexpr (MASK && !I8) {
-                    // tokens that no row of this wave sees may hold anything, also NaN
-                    keep = keep_words(w.skip[j] ? 0u : seen_bits(t0[j] + 16 * g + 8 * hk, wlow, w_hi, t.pre, 8));
-                }
+                if constexpr (MASK && !I8) keep = keep_of(j, g);
 #pragma unroll
                 for (int d = 0; d < DT; d++) {
                     frag va;
@@ -888,8 +974,17 @@ __global__ __launch_bounds__(PF_WAVES * 64, 2) void paged_prompt_kernel(PagedAtt
                         const uint2 vw = *(const uint2*)(vb + j * BLK + v_lane + d * 1024 + g * 512);
                         va = i8_to_half8(vw.x, vw.y);
                     } else {
-                        u32x4_t vw = *(const u32x4_t*)(vb + j * BLK + (v_lane ^ (g * 32)) + d * 2048);
-                        if constexpr (MASK) vw &= keep;
+                        u32x4_t vw = v_at(j, g, d);
+                        if constexpr (MASK) {
+                            vw &= keep;
+                            if (__builtin_expect(odd, 0)) {
+                                const frag seen = Odd<KVF>::seen(w.skip[j] ? 0u : seen_bits(t0[j] + 16 * g + 8 * hk, a.window ? max(0, pos - a.window + 1) : 0, pos, t.pre, 8));
+                                const float16_t c = mfma32<KVF>(Odd<KVF>::marks(vw), seen, float16_t{});
+#pragma unroll
+                                for (int i = 0; i < 16; i++) o[d][i] += Odd<KVF>::worth(c[i]);
+                                vw = Odd<KVF>::finite(vw);
+                            }
+                        }
                         va = __builtin_bit_cast(frag, vw);
                     }
                     o[d] = mfma32<KVF>(va, ph, o[d]);

@@ -436,8 +436,9 @@ int aarh_rope_frequencies(int32_t rot_dim, double theta, int32_t max_seq_len, co
    key j and row position p.  Key j < kv_len is visible if j <= p and (window = 0 or p - j < window),
    or if j < prefix[b].  out = softmax(score) v over the visible keys, zero where there are none.
    Query head h reads kv head h % n_kv_heads (the reference's map), or h / (n_heads /
-   n_kv_heads) with grouped = 1.  Types as for aarh_rope_append; out has q's type.  A key that no row
-   of a call sees may hold anything; one that some row sees must be finite.
+   n_kv_heads) with grouped = 1.  Types as for aarh_rope_append; out has q's type.  Tokens
+   that a row does not see may hold anything, infinities and NaN too: they do not reach that row (a row that sees one gets
+   a result that is not finite).
    Query heads of a kv head are taken together; a call whose sequences have like numbers of rows is quickest (the grid is
    made for max_rows and max_kv: give prompts and single tokens calls of their own).  nseq x n_kv_heads x (max_rows x n_heads /
    n_kv_heads / 128 + 1) is at most 2^23 (SHAPE otherwise).

@@ -174,6 +174,58 @@ def test_a_captured_decode_step(ctx):
         assert torch.equal(a.view(torch.int16), b.view(torch.int16))
 
 
+@pytest.mark.parametrize("act,kv", TYPES)
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("wide,how", [(False, {}), (False, dict(window=6)), (True, {}), (True, dict(window=20, prefix=[0, 3])),
+                                      (False, dict(prefix=[9, 0]))])
+def test_infinities_and_nan_reach_only_the_rows_that_see_them(ctx, act, kv, hd, wide, how):
+    """Keys and values of tokens that some rows of a call see and others, beside them in a tile, do not."""
+    rows = [60, 45] if wide else [7, 5]
+    lens = [75, 45 + 64]
+    cache = U.Cache(np.random.default_rng(128), kv, 2, hd, 32, lens)
+    inf, nan = float("inf"), float("nan")
+
+    def plant(which, b, tok, h, dim, value):
+        page, at = int(cache.tables[b, tok // 32]), tok % 32
+        if kv == "int8":
+            cache.st[which][page, h, at] = value
+        else:
+            cache.t[which][page, h, int((cache.v_at if which else cache.k_at)[at, dim])] = value
+
+    # 16-bit pools: single elements; INT8: a token's scale.  (row of the token, kv head, dimension, value)
+    r0 = [n - r for n, r in zip(lens, rows)]
+    plant(1, 0, r0[0] + 3, 0, 5, inf)
+    plant(1, 0, r0[0] + 5, 0, hd - 1, nan)
+    plant(1, 0, r0[0] + 5, 1, 17, -inf)
+    plant(1, 1, r0[1] + 2, 1, 40, -inf)
+    plant(1, 1, r0[1] + 4, 1, 40, inf)
+    plant(0, 1, r0[1] + 3, 0, 8, nan)
+    nh = 8
+    q = torch.randn((sum(rows), nh, hd), device=DEV, generator=torch.Generator(DEV).manual_seed(3)).to(U.DT[act])
+    args = dict(how)
+    if "prefix" in args:
+        args["prefix"] = torch.tensor(args["prefix"], dtype=torch.int32, device=DEV)
+    bt = cache.batch(rows, max_kv=much(rows, 2, nh, hd, kv) if wide else None)
+    if wide:
+        table = torch.full((2, bt._c.max_kv // 32 + 1), -1, dtype=torch.int32, device=DEV)
+        table[:, :cache.tables.shape[1]] = bt.tables
+        bt = A.PageBatch(table, bt.kv_len, bt.row_off, rows=sum(rows), max_rows=max(rows), max_kv=bt._c.max_kv)
+    got = f64(ctx.paged_attention(cache.pool, bt, q, **args))
+    with np.errstate(invalid="ignore"):
+        want, mag, err = U.attention_reference(cache, f64(q), rows, hd ** -0.5, **how)
+        fine = np.isfinite(want)
+        assert 0 < fine.sum() < fine.size
+        bound = U.attention_bound(want, mag, err, act, kv, max(lens))
+        assert np.all(np.isfinite(got[fine]))
+        off = np.abs(got - want)
+        live = fine & np.isfinite(bound)
+        assert np.all(off[live] <= bound[live]), (off[live] / bound[live]).max()
+        assert not np.any(np.isfinite(got[~fine]))
+        # (f32 rows have weights of two halves, of which the second may be zero or negative: with an infinity that makes NaN)
+        if kv != "int8" and act != "f32":
+            assert np.array_equal(got[~fine], want[~fine], equal_nan=True)
+
+
 def test_grids_past_their_bound_are_refused(ctx):
     pool = A.PagePool.allocate(1, 8, 64, 32)
     n, rows = 60000, 2300
