@@ -10,6 +10,13 @@
 // Running maximum, sum and O are f32.  P is rounded to the pool's 16 bits for the product with V
 // (2^-11 or 2^-8 of each weight, as V itself was); f32 queries are split into fp16 hi + lo
 // halves, and so is P (2^-22 together): two matrix instructions in place of one.
+//
+// Few rows (paged_decode_kernel): bound by the cache's bytes, one pass, the cache split over the compute units and joined
+// by a second launch; in short calls by that chain of launches and loads.  Many rows (paged_prompt_kernel): bound by the matrix
+// instructions at the clock that the power budget leaves (fp16 runs 6% slower than bf16 with the same instructions).
+// Measured, 32 query heads on 8 of size 128: one token over 4096 fp16 10 us (two launches); 16 tokens over 32768 bf16
+// 258 us (6.4 TB/s); 32 x 4 rows over 4096 INT8, f32, 51 us (4.1 TB/s); 8192 rows bf16 552 us (1.0 PFLOP/s), with a cap and
+// a window of 4096 532 us; 500 rows behind 3000 fp16 58 us.
 #include <algorithm>
 #include <cmath>
 #include <type_traits>
