@@ -385,7 +385,7 @@ def _on(device, name, t, dtype, dim, contiguous=True):
     """Data pointer of a device tensor (None: NULL) after its checks."""
     if t is None:
         return None
-    if not t.is_cuda or t.get_device() != device:
+    if t.get_device() != device:  # (-1 for the CPU)
         raise ConfigError(f"{name} must be on cuda:{device}, not {t.device}")
     if t.dtype != dtype:
         raise UnsupportedError(f"{name} must be {dtype}, not {t.dtype}")
@@ -394,6 +394,15 @@ def _on(device, name, t, dtype, dim, contiguous=True):
     if contiguous and not t.is_contiguous():
         raise UnsupportedError(f"{name} must be contiguous")
     return t.data_ptr()
+
+
+def _sized(device, name, t, dtype, shape):
+    """Data pointer of a contiguous device tensor of one shape (None: NULL) after its checks."""
+    if t is None:
+        return None
+    if t.shape != shape:
+        raise ShapeError(f"{name} must be {shape}, not {tuple(t.shape)}")
+    return _on(device, name, t, dtype, len(shape))
 
 
 def _stream(device):
@@ -407,6 +416,12 @@ def _raw_stream():
     import torch
     return getattr(torch._C, "_cuda_getCurrentRawStream", None) or \
         (lambda device: torch.cuda.current_stream(device).cuda_stream)
+
+
+@functools.lru_cache(None)
+def _types():
+    import torch
+    return torch.float64, torch.float32, torch.int32
 
 
 @functools.lru_cache(None)
@@ -824,7 +839,7 @@ class HipModel:
         act = _act_formats().get(t.dtype)
         if act is None:
             raise UnsupportedError(f"{name} must be float32, float16 or bfloat16, not {t.dtype}")
-        if not t.is_cuda or t.get_device() != self.device:
+        if t.get_device() != self.device:
             raise ConfigError(f"{name} must be on cuda:{self.device}, not {t.device}")
         if t.shape != (rows, heads, hd):
             raise ShapeError(f"{name} must be {(rows, heads, hd)}, not {tuple(t.shape)}")
@@ -844,7 +859,6 @@ class HipModel:
         """Rotary positions of the call's rows and their append to the pages (aarh_rope_append): q [rows, n_heads,
         head_dim] or None, k, v [rows, n_kv_heads, head_dim], whose rows may be apart (views of a fused
         projection); inv_freq [rot_dim / 2] float64 (None: no rotation).  Returns the rotated queries."""
-        import torch
         self._paged(pool, batch)
         n, hd = batch.rows, pool.head_dim
         act, k_ld = self._act("k", k, n, pool.n_kv_heads, hd)
@@ -861,7 +875,7 @@ class HipModel:
                 raise UnsupportedError("q, k, v and out must have one type")
         if v_act != act:
             raise UnsupportedError("q, k, v and out must have one type")
-        f = _on(self.device, "inv_freq", inv_freq, torch.float64, 1)
+        f = _on(self.device, "inv_freq", inv_freq, _types()[0], 1)
         a = _RopeArgs(act, heads, None if q is None else q.data_ptr(), k.data_ptr(), v.data_ptr(), q_ld, k_ld, v_ld,
                       None if q is None else out.data_ptr(), o_ld, f, 0 if inv_freq is None else 2 * inv_freq.shape[0],
                       1 if interleaved else 0, attn_factor)
@@ -885,10 +899,11 @@ class HipModel:
             o_act, o_ld = self._act("out", out, n, heads, hd)
             if o_act != act:
                 raise UnsupportedError("q and out must have one type")
-        sl = _on(self.device, "slopes", slopes, torch.float32, 1)
-        pre = _on(self.device, "prefix", prefix, torch.int32, 1)
-        if (slopes is not None and slopes.shape[0] != heads) or (prefix is not None and prefix.shape[0] != batch._c.nseq):
-            raise ShapeError("slopes has a value for each head, prefix one for each sequence")
+        sl = pre = None
+        if slopes is not None:
+            sl = _sized(self.device, "slopes", slopes, _types()[1], (heads,))
+        if prefix is not None:
+            pre = _sized(self.device, "prefix", prefix, _types()[2], (batch._c.nseq,))
         a = _PagedAttnArgs(act, heads, 1 if grouped else 0, q.data_ptr(), q_ld, out.data_ptr(), o_ld,
                            hd ** -0.5 if scale is None else scale, softcap, window, sl, pre, None, 0)
         key = (act, heads, window, pre is None, pool.kv_format, pool.n_kv_heads, hd, pool.page_tokens)
@@ -914,22 +929,18 @@ class HipModel:
         (repetition, presence, frequency), draft [nseq, rows_per_seq - 1] int32 proposals, biases as bias_off
         [nseq + 1] into bias_ids / bias_vals, masks [n, ceil(vocab / 32)] int32 bits and mask_of_row.
         out may be logits (in place).  Returns the processed rows."""
-        import torch
         if rows_per_seq <= 0 or logits.dim() != 2 or logits.shape[0] % rows_per_seq:
             raise ShapeError(f"logits {tuple(logits.shape)} are not rows of {rows_per_seq} for each sequence")
         rows, V = logits.shape
-        n, dev, i32, f32 = rows // rows_per_seq, self.device, torch.int32, torch.float32
-        for name, t in (("logits", logits), ("out", out)):
-            _on(dev, name, t, f32, 2, contiguous=False)
-            if t is not None and (t.shape != (rows, V) or (V > 1 and t.stride(1) != 1)):
-                raise UnsupportedError(f"{name} must be {(rows, V)} with contiguous rows")
+        n, dev, (_, f32, i32) = rows // rows_per_seq, self.device, _types()
+        x, y = _on(dev, "logits", logits, f32, 2, contiguous=False), None
         if out is None:
             out = logits.new_empty((rows, V))
-        for name, t, shape in (("history_len", history_len, (n,)), ("prompt_len", prompt_len, (n,)),
-                               ("penalties", penalties, (n, 3)), ("bias_off", bias_off, (n + 1,)),
-                               ("mask_of_row", mask_of_row, (rows,))):
-            if t is not None and t.shape != shape:
-                raise ShapeError(f"{name} must be {shape}, not {tuple(t.shape)}")
+            y, out_ld = out.data_ptr(), V
+        else:
+            y, out_ld = _on(dev, "out", out, f32, 2, contiguous=False), out.stride(0) if rows > 1 else V
+        if out.shape != (rows, V) or (V > 1 and (logits.stride(1) != 1 or out.stride(1) != 1)):
+            raise UnsupportedError(f"logits and out must be {(rows, V)} with contiguous rows")
         if (history is not None and history.shape[0] != n) or (draft is not None and draft.shape[0] != n):
             raise ShapeError(f"history and draft must have a row for each of {n} sequences")
         if draft is not None and draft.shape[1] < rows_per_seq - 1:
@@ -940,15 +951,26 @@ class HipModel:
             raise ShapeError("bias_ids and bias_vals must have one length")
         if bias_off is not None and bias_ids is None:
             raise ConfigError("bias_off needs bias_ids and bias_vals")
-        a = _LogitsArgs(n, rows_per_seq, V, logits.data_ptr(), logits.stride(0) if rows > 1 else V, out.data_ptr(),
-                        out.stride(0) if rows > 1 else V, _on(dev, "history", history, i32, 2),
-                        0 if history is None else history.shape[1], _on(dev, "history_len", history_len, i32, 1),
-                        _on(dev, "prompt_len", prompt_len, i32, 1), _on(dev, "penalties", penalties, f32, 2),
-                        _on(dev, "draft", draft, i32, 2), 0 if draft is None else draft.shape[1],
-                        _on(dev, "bias_off", bias_off, i32, 1), _on(dev, "bias_ids", bias_ids, i32, 1),
-                        _on(dev, "bias_vals", bias_vals, f32, 1), 0 if bias_ids is None else bias_ids.shape[0],
-                        _on(dev, "masks", masks, i32, 2), 0 if masks is None else masks.shape[1],
-                        0 if masks is None else masks.shape[0], _on(dev, "mask_of_row", mask_of_row, i32, 1))
+        a = _LogitsArgs(n, rows_per_seq, V, x, logits.stride(0) if rows > 1 else V, y, out_ld)
+        if history is not None:
+            a.history, a.history_ld = _on(dev, "history", history, i32, 2), history.shape[1]
+        if history_len is not None:
+            a.history_len = _sized(dev, "history_len", history_len, i32, (n,))
+        if prompt_len is not None:
+            a.prompt_len = _sized(dev, "prompt_len", prompt_len, i32, (n,))
+        if penalties is not None:
+            a.penalties = _sized(dev, "penalties", penalties, f32, (n, 3))
+        if draft is not None:
+            a.draft, a.draft_ld = _on(dev, "draft", draft, i32, 2), draft.shape[1]
+        if bias_off is not None:
+            a.bias_off = _sized(dev, "bias_off", bias_off, i32, (n + 1,))
+        if bias_ids is not None:
+            a.bias_ids, a.bias_vals = _on(dev, "bias_ids", bias_ids, i32, 1), _on(dev, "bias_vals", bias_vals, f32, 1)
+            a.n_bias = bias_ids.shape[0]
+        if masks is not None:
+            a.masks, a.mask_ld, a.n_masks = _on(dev, "masks", masks, i32, 2), masks.shape[1], masks.shape[0]
+        if mask_of_row is not None:
+            a.mask_of_row = _sized(dev, "mask_of_row", mask_of_row, i32, (rows,))
         st = lib().aarh_process_logits(self.h, a, _stream(dev))
         if st:
             self._check(st)
