@@ -247,3 +247,32 @@ def test_many_rows_over_a_few_splits(ctx, act, kv, hd, rows, lens):
     assert torch.equal(ctx.paged_attention(cache.pool, bt, q), out)
     splits = next(iter(bt._workspace.values())) / (sum(rows) * 32 * (hd + 2) * 4)
     assert 2 <= splits <= 512 // hd, splits
+
+
+def test_calls_from_two_threads(ctx):
+    """One context, two threads with streams and batches of their own: the results of calls one after another."""
+    import threading
+    made = []
+    for seed in (129, 130):
+        cache = U.Cache(np.random.default_rng(seed), "f16", 2, 64, 32, [400, 90])
+        q = torch.randn((6, 8, 64), device=DEV, generator=torch.Generator(DEV).manual_seed(seed)).half()
+        want = ctx.paged_attention(cache.pool, cache.batch([3, 3]), q)
+        made.append((cache, q, want, []))
+    torch.cuda.synchronize()
+
+    def work(cache, q, want, got):
+        stream = torch.cuda.Stream()
+        with torch.cuda.stream(stream):
+            bt = cache.batch([3, 3])
+            stream.synchronize()
+            for _ in range(50):
+                got.append(ctx.paged_attention(cache.pool, bt, q))
+        stream.synchronize()
+
+    threads = [threading.Thread(target=work, args=m) for m in made]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    for _, _, want, got in made:
+        assert len(got) == 50 and all(torch.equal(g, want) for g in got)
