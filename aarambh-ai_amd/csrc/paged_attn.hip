@@ -638,10 +638,12 @@ __device__ __forceinline__ float half_sum(float x) {
 __device__ __forceinline__ void lds_piece(__amdgpu_buffer_rsrc_t r, const void* lds_dst, int voff, int soff, int i) {
     const unsigned base = __builtin_amdgcn_readfirstlane((unsigned)(uintptr_t)lds_dst);
     switch (i) {
-        case 0: asm volatile("s_nop 0\n\tbuffer_load_dwordx4 %0, %1, %2 offen lds" ::"v"(voff), "s"(r), "s"(soff), "{m0}"(base) : "memory"); break;
-        case 1: asm volatile("s_nop 0\n\tbuffer_load_dwordx4 %0, %1, %2 offen offset:1024 lds" ::"v"(voff), "s"(r), "s"(soff), "{m0}"(base) : "memory"); break;
-        case 2: asm volatile("s_nop 0\n\tbuffer_load_dwordx4 %0, %1, %2 offen offset:2048 lds" ::"v"(voff), "s"(r), "s"(soff), "{m0}"(base) : "memory"); break;
-        default: asm volatile("s_nop 0\n\tbuffer_load_dwordx4 %0, %1, %2 offen offset:3072 lds" ::"v"(voff), "s"(r), "s"(soff), "{m0}"(base) : "memory"); break;
+#define AARH_PIECE(N) asm volatile("s_nop 0\n\tbuffer_load_dwordx4 %0, %1, %2 offen offset:%3 lds" ::"v"(voff), "s"(r), "s"(soff), "n"((N) * 1024), "{m0}"(base) : "memory")
+        case 0: AARH_PIECE(0); break;
+        case 1: AARH_PIECE(1); break;
+        case 2: AARH_PIECE(2); break;
+        default: AARH_PIECE(3); break;
+#undef AARH_PIECE
     }
 }
 
